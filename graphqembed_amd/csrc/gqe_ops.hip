@@ -1,0 +1,391 @@
+// gqe_ops.hip — the operators of include/gqe_ops.h: entry points, the joins of the softmax cross entropy's splits, gradient norm and
+// clipping, layer normalisation.  The softmax cross entropy's two passes are gqe_xent.h.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdio.h>
+
+#include <algorithm>
+#include <string>
+#include <vector>
+
+#include "../../include/gqe_ops.h"
+#include "gqe_common.h"
+#include "gqe_ops_dev.h"
+#include "gqe_xent.h"
+
+namespace {
+
+thread_local std::string g_ops_error;
+
+int refuse(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  try {
+    g_ops_error = buf;
+  } catch (...) {
+  }
+  return code;
+}
+
+// the launches of a call go to `device`, whatever device the caller has current
+struct OnDevice {
+  int before = -1;
+  hipError_t status;
+  explicit OnDevice(int device) {
+    status = hipGetDevice(&before);
+    if (status == hipSuccess && before != device) status = hipSetDevice(device);
+    else if (status == hipSuccess) before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+int hip_refuse(hipError_t e, const char* what) { return refuse(GQE_ERR_HIP, "%s: %s", what, hipGetErrorString(e)); }
+
+int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
+
+bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+
+// ------------------------------------------------------------------------------------------------------------------------------
+// softmax cross entropy: join of the splits
+// ------------------------------------------------------------------------------------------------------------------------------
+#define XENT_MAX_SPLIT 1024
+
+struct XentJoin {
+  const float *part_m, *part_l, *part_o, *st;
+  int32_t n_split, ny, d, n_rows;
+  const int32_t* target;
+  const float* weight;
+  const void* table;       // DQ: the target's row; DT: the row itself
+  int64_t table_stride;
+  int32_t unit, out_f32, accumulate;
+  float scale;
+  float *loss, *lse, *stat;
+  void* out;
+  int64_t out_stride;
+};
+
+template <bool BF16>
+__device__ __forceinline__ float row_elem(const void* p, int64_t i) {
+  if (BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
+  return ((const float*)p)[i];
+}
+template <bool BF16>
+__device__ __forceinline__ void put_elem(void* p, int64_t i, float v, bool accumulate) {
+  if (BF16) {
+    ((uint16_t*)p)[i] = (uint16_t)xent_pack_bf16(v, v);
+  } else {
+    float* q = (float*)p + i;
+    *q = accumulate ? *q + v : v;
+  }
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return x;
+}
+__device__ __forceinline__ double wave_sum_f64(double x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+// One workgroup of WAVES waves per stationary row: the splits' sums brought to one unit and added in a fixed order.  What it reads is
+// n_split rows of partial sums; their latency is hidden by the many rows in flight.
+template <bool BF16, int MODE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
+  __shared__ float ws[MODE == XENT_MODE_LSE ? 1 : XENT_MAX_SPLIT];
+  __shared__ double red[WAVES];
+  __shared__ float redf[WAVES];
+  __shared__ float acc[WAVES][256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t y = blockIdx.x;
+  float m = XENT_NONE;
+  for (int s = tid; s < p.n_split; s += 64 * WAVES) m = fmaxf(m, p.part_m[(int64_t)s * p.ny + y]);
+  m = wave_max(m);
+  if (WAVES > 1) {
+    if (lane == 0) redf[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, redf[w]);
+  }
+  float half = 0.f, f = 0.f, share = 0.f, g = 0.f;      // half * f: the unit's power in two factors, the sums carry the operands' 2^30
+  int tg = -1;
+  if (MODE != XENT_MODE_DT) {
+    double l = 0.0;
+    for (int s = tid; s < p.n_split; s += 64 * WAVES)
+      l += (double)p.part_l[(int64_t)s * p.ny + y] * (double)exp2f(p.part_m[(int64_t)s * p.ny + y] - m);
+    l = wave_sum_f64(l);
+    if (WAVES > 1) {
+      if (lane == 0) red[wave] = l;
+      __syncthreads();
+      l = 0.0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) l += red[w];
+    }
+    tg = p.target[y];
+    const bool has = tg >= 0 && tg < p.n_rows;
+    const double others = (double)m + log2(l);              // -inf where the target is the only row
+    double lse2 = others, lr = 0.0, loss = 0.0;
+    if (has) {
+      const double diff = others - (double)p.st[y];          // log2 of (sum of the others / the target's term)
+      const double soft = log1p(exp2(-fabs(diff))) * 1.4426950408889634;
+      lse2 = fmax(others, (double)p.st[y]) + soft;
+      if (diff != diff) lse2 = diff;
+      loss = (fmax(diff, 0.0) + soft) * 0.6931471805599453;
+      lr = fmin(diff, 0.0) - soft;
+      if (diff != diff) loss = lr = diff;
+    } else if (tg >= p.n_rows) {
+      loss = __longlong_as_double(0x7ff8000000000000LL);
+    }
+    g = has ? (p.weight ? p.weight[y] : 1.f) : 0.f;
+    if (tid == 0) {
+      if (p.loss) p.loss[y] = (float)loss;
+      if (p.lse) p.lse[y] = (float)(lse2 * 0.6931471805599453);
+      p.stat[2 * y] = (float)lse2;
+      p.stat[2 * y + 1] = (float)lr;
+    }
+    if (MODE == XENT_MODE_LSE) return;
+    if (!has) tg = -1;
+    share = (float)exp2(lr);
+    half = f = (float)exp2(0.5 * ((double)m - lse2));
+  } else {
+    half = exp2f(0.5f * m);
+    f = p.scale * half;
+  }
+  for (int s = tid; s < p.n_split; s += 64 * WAVES) ws[s] = exp2f(p.part_m[(int64_t)s * p.ny + y] - m);
+  __syncthreads();
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const int64_t step = (int64_t)p.ny * p.d;
+  const float* po = p.part_o + y * p.d + lane;
+#pragma unroll 4
+  for (int s = wave; s < p.n_split; s += WAVES) {
+    const float w = ws[s];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (lane + 64 * c < p.d) v[c] = fmaf(w, po[s * step + 64 * c], v[c]);
+  }
+  if (WAVES > 1) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[wave][lane + 64 * c] = v[c];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v[c] += acc[w][lane + 64 * c];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] = v[c] * half * f;
+  const int64_t row = MODE == XENT_MODE_DT ? y : tg;
+  float t[4] = {0.f, 0.f, 0.f, 0.f}, rn = 1.f;
+  if (row >= 0 && (MODE == XENT_MODE_DQ || p.unit)) {
+    float mx = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (lane + 64 * c < p.d) {
+        t[c] = row_elem<BF16>(p.table, row * p.table_stride + lane + 64 * c);
+        mx = fmaxf(mx, fabsf(t[c]));
+      }
+    if (p.unit) {
+      const float k = xent_pow2(xent_row_scale(wave_max(mx)));
+      float ss = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) ss = fmaf(t[c] * k, t[c] * k, ss);
+      ss = wave_sum(ss);
+      rn = ss > 0.f ? k / sqrtf(ss) : (ss == 0.f ? 0.f : ss);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) t[c] *= rn;
+    }
+  }
+  if (MODE == XENT_MODE_DQ) {
+    const float gs = g * p.scale;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = g != 0.f ? gs * fmaf(-share, t[c], v[c]) : 0.f;
+  } else if (p.unit) {
+    float along = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) along = fmaf(t[c], v[c], along);
+    along = wave_sum(along);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = (v[c] - t[c] * along) * rn;
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (lane + 64 * c < p.d) {
+      if (p.out_f32) put_elem<false>(p.out, y * p.out_stride + lane + 64 * c, v[c], p.accumulate != 0);
+      else put_elem<BF16>(p.out, y * p.out_stride + lane + 64 * c, v[c], p.accumulate != 0);
+    }
+}
+
+struct XentPlan {
+  int dk, n_tiles, n_yblk, n_split, per;
+};
+
+// Splits of the streamed axis: enough workgroups to fill the 256 CUs (`slots` of them at once), never more splits than tiles.
+XentPlan xent_plan(int64_t ny, int64_t nx, int dim, int slots) {
+  XentPlan r;
+  r.dk = dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
+  r.n_tiles = (int)((nx + XENT_TR - 1) / XENT_TR);
+  r.n_yblk = (int)((ny + XENT_BM - 1) / XENT_BM);
+  int64_t s = std::max<int64_t>(1, slots / std::max(r.n_yblk, 1));
+  s = std::min<int64_t>(std::min<int64_t>(s, XENT_MAX_SPLIT), std::max(r.n_tiles, 1));
+  r.per = std::max(1, (int)((r.n_tiles + s - 1) / s));
+  r.n_split = std::max(1, (r.n_tiles + r.per - 1) / r.per);
+  return r;
+}
+int xent_slots(int dim) { return dim <= 128 ? 512 : 256; }
+
+struct XentSpace {
+  int64_t part_m, part_l, st, stat, part_o, total;
+};
+XentSpace xent_space(const gqe_xent_args* a, const XentPlan& q, const XentPlan& t) {
+  XentSpace s;
+  const bool dq = a->phase & GQE_XENT_DQ, dt = (a->phase & GQE_XENT_DTABLE) && t.n_split > 1;
+  const bool first = a->phase & (GQE_XENT_LOSS | GQE_XENT_DQ);
+  const int64_t pq = first ? (int64_t)q.n_split * a->n_queries : 0, pt = dt ? (int64_t)t.n_split * a->n_rows : 0;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { const int64_t o = at; at = up(at + bytes, 256); return o; };
+  s.part_m = take(4 * std::max(pq, pt));
+  s.part_l = take(4 * pq);
+  s.st = take(first ? 4 * a->n_queries : 0);
+  s.stat = take(a->stat ? 0 : 8 * a->n_queries);
+  s.part_o = take(4 * (int64_t)a->dim * std::max(dq ? pq : 0, pt));
+  s.total = at;
+  return s;
+}
+
+hipError_t xent_launch(bool bf16, int dk, int mode, const XentPass& p, hipStream_t s) {
+  switch (dk) {
+    case 64: return bf16 ? gqe_xent_launch_1_64(mode, p, s) : gqe_xent_launch_0_64(mode, p, s);
+    case 128: return bf16 ? gqe_xent_launch_1_128(mode, p, s) : gqe_xent_launch_0_128(mode, p, s);
+    case 192: return bf16 ? gqe_xent_launch_1_192(mode, p, s) : gqe_xent_launch_0_192(mode, p, s);
+    default: return bf16 ? gqe_xent_launch_1_256(mode, p, s) : gqe_xent_launch_0_256(mode, p, s);
+  }
+}
+
+template <int MODE>
+void join_launch(bool bf16, const XentJoin& j, hipStream_t s) {
+  const dim3 grid((unsigned)j.ny);
+  if (j.n_split > 4) {
+    if (bf16) gqe_xent_join_kernel<true, MODE, 4><<<grid, dim3(256), 0, s>>>(j);
+    else gqe_xent_join_kernel<false, MODE, 4><<<grid, dim3(256), 0, s>>>(j);
+  } else {
+    if (bf16) gqe_xent_join_kernel<true, MODE, 1><<<grid, dim3(64), 0, s>>>(j);
+    else gqe_xent_join_kernel<false, MODE, 1><<<grid, dim3(64), 0, s>>>(j);
+  }
+}
+
+// sizes alone: what the workspace depends on
+int xent_check_sizes(const gqe_xent_args* a) {
+  if (!a) return refuse(GQE_ERR_ARG, "softmax_xent: args is NULL");
+  if (a->phase < 1 || a->phase > 7) return refuse(GQE_ERR_ARG, "softmax_xent: phase %d", a->phase);
+  if (a->dtype != GQE_F32 && a->dtype != GQE_BF16) return refuse(GQE_ERR_ARG, "softmax_xent: dtype %d is neither float32 nor bfloat16", a->dtype);
+  if (a->dim < 1 || a->dim > GQE_MAX_DIM) return refuse(GQE_ERR_ARG, "softmax_xent: dim %d is not in 1 .. %d", a->dim, GQE_MAX_DIM);
+  if (a->n_rows < 1 || a->n_rows > 0x7fffff00LL) return refuse(GQE_ERR_ARG, "softmax_xent: a table of %lld rows", (long long)a->n_rows);
+  if (a->n_queries < 0 || a->n_queries > 0x7fffff00LL) return refuse(GQE_ERR_ARG, "softmax_xent: %lld queries", (long long)a->n_queries);
+  return GQE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* gqe_ops_last_error(void) { return g_ops_error.c_str(); }
+
+int64_t gqe_softmax_xent_workspace(const gqe_xent_args* a) {
+  const int rc = xent_check_sizes(a);
+  if (rc) return rc;
+  const XentPlan q = xent_plan(a->n_queries, a->n_rows, a->dim, xent_slots(a->dim));
+  const XentPlan t = xent_plan(a->n_rows, a->n_queries, a->dim, xent_slots(a->dim));
+  return std::max<int64_t>(256, xent_space(a, q, t).total);
+}
+
+int gqe_softmax_xent(const gqe_xent_args* a) {
+  int rc = xent_check_sizes(a);
+  if (rc) return rc;
+  const bool first = a->phase & (GQE_XENT_LOSS | GQE_XENT_DQ), dq = a->phase & GQE_XENT_DQ, dt = a->phase & GQE_XENT_DTABLE;
+  const bool bf16 = a->dtype == GQE_BF16;
+  const int64_t B = a->n_queries, V = a->n_rows;
+  const size_t esize = bf16 ? 2 : 4;
+  if (!a->table || (B && (!a->q || !a->target))) return refuse(GQE_ERR_ARG, "softmax_xent: q, table or target is NULL");
+  if (dq && B && !a->dq) return refuse(GQE_ERR_ARG, "softmax_xent: dq is NULL");
+  if (dt && !a->dtable) return refuse(GQE_ERR_ARG, "softmax_xent: dtable is NULL");
+  if (dt && !first && B && !a->stat) return refuse(GQE_ERR_ARG, "softmax_xent: the table's gradient alone needs stat of an earlier call");
+  if (a->accumulate && bf16) return refuse(GQE_ERR_ARG, "softmax_xent: accumulate needs a float32 table");
+  if (!isfinite(a->scale)) return refuse(GQE_ERR_ARG, "softmax_xent: scale is not finite");
+  if (a->table_stride < a->dim || (B > 1 && a->q_stride < a->dim) || (dt && a->dtable_stride < a->dim) || (dq && B > 1 && a->dq_stride < a->dim))
+    return refuse(GQE_ERR_ARG, "softmax_xent: a row stride is smaller than dim %d", a->dim);
+  if (!aligned(a->q, esize) || !aligned(a->table, esize) || !aligned(a->dq, a->dq_f32 ? 4 : esize) || !aligned(a->dtable, esize))
+    return refuse(GQE_ERR_ARG, "softmax_xent: a pointer is not aligned to its element");
+  const XentPlan pq = xent_plan(B, V, a->dim, xent_slots(a->dim)), pt = xent_plan(V, B, a->dim, xent_slots(a->dim));
+  const XentSpace sp = xent_space(a, pq, pt);
+  if (a->workspace_bytes < sp.total || (sp.total && (!a->workspace || !aligned(a->workspace, 256))))
+    return refuse(GQE_ERR_WORKSPACE, "softmax_xent: needs %lld workspace bytes, 256-byte aligned; got %lld", (long long)sp.total, (long long)a->workspace_bytes);
+  OnDevice dev(a->device);
+  if (dev.status != hipSuccess) return hip_refuse(dev.status, "softmax_xent");
+  hipStream_t stream = (hipStream_t)a->stream;
+  char* w = (char*)a->workspace;
+  const int vec = bf16 ? 8 : 4;
+  const bool dvec = a->dim % 8 == 0;
+  const auto rows_vec = [&](const void* ptr, int64_t stride) { return dvec && aligned(ptr, 16) && stride % vec == 0; };
+
+  XentPass p = {};
+  p.d = a->dim;
+  p.scale2 = (float)((double)a->scale * 1.4426950408889634);
+  p.scale = a->scale;
+  p.target = a->target;
+  p.part_m = (float*)(w + sp.part_m);
+  p.part_l = (float*)(w + sp.part_l);
+  p.part_o = (float*)(w + sp.part_o);
+  p.st = (float*)(w + sp.st);
+  float* stat = a->stat ? a->stat : (float*)(w + sp.stat);
+  p.stat = stat;
+  XentJoin j = {};
+  j.part_m = p.part_m; j.part_l = p.part_l; j.part_o = p.part_o; j.st = p.st;
+  j.d = a->dim; j.n_rows = (int32_t)V; j.target = a->target; j.weight = a->weight;
+  j.table = a->table; j.table_stride = a->table_stride; j.unit = a->normalize ? 1 : 0; j.scale = a->scale;
+  if (first && B) {
+    p.y = a->q; p.y_stride = a->q_stride; p.ny = (int32_t)B; p.y_vec = rows_vec(a->q, a->q_stride);
+    p.x = a->table; p.x_stride = a->table_stride; p.nx = (int32_t)V; p.x_vec = rows_vec(a->table, a->table_stride);
+    p.x_unit = a->normalize ? 1 : 0;
+    p.n_tiles = pq.n_tiles; p.tiles_per_split = pq.per; p.n_split = pq.n_split; p.n_yblk = pq.n_yblk;
+    hipError_t e = xent_launch(bf16, pq.dk, dq ? XENT_MODE_DQ : XENT_MODE_LSE, p, stream);
+    if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
+    j.n_split = pq.n_split; j.ny = (int32_t)B;
+    j.loss = a->loss; j.lse = a->lse; j.stat = stat;
+    j.out = a->dq; j.out_stride = a->dq_stride; j.out_f32 = a->dq_f32 || !bf16;
+    if (dq) join_launch<XENT_MODE_DQ>(bf16, j, stream);
+    else join_launch<XENT_MODE_LSE>(bf16, j, stream);
+    if ((e = hipGetLastError()) != hipSuccess) return hip_refuse(e, "softmax_xent");
+  }
+  if (dt) {
+    p.y = a->table; p.y_stride = a->table_stride; p.ny = (int32_t)V; p.y_vec = rows_vec(a->table, a->table_stride); p.y_unit = a->normalize ? 1 : 0;
+    p.x = a->q; p.x_stride = a->q_stride; p.nx = (int32_t)B; p.x_vec = rows_vec(a->q, a->q_stride); p.x_unit = 0;
+    p.weight = a->weight;
+    p.n_tiles = pt.n_tiles; p.tiles_per_split = pt.per; p.n_split = pt.n_split; p.n_yblk = pt.n_yblk;
+    p.out = a->dtable; p.out_stride = a->dtable_stride; p.accumulate = a->accumulate;
+    p.out_vec = a->dim % 4 == 0 && aligned(a->dtable, bf16 ? 8 : 16) && a->dtable_stride % 4 == 0;
+    hipError_t e = xent_launch(bf16, pt.dk, XENT_MODE_DT, p, stream);
+    if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
+    if (pt.n_split > 1) {
+      j.n_split = pt.n_split; j.ny = (int32_t)V;
+      j.out = a->dtable; j.out_stride = a->dtable_stride; j.out_f32 = !bf16; j.accumulate = a->accumulate;
+      join_launch<XENT_MODE_DT>(bf16, j, stream);
+      if ((e = hipGetLastError()) != hipSuccess) return hip_refuse(e, "softmax_xent");
+    }
+  }
+  return GQE_OK;
+}
+
+}  // extern "C"
+
+#include "gqe_clip.h"
+#include "gqe_layer_norm.h"
