@@ -262,12 +262,12 @@ XentSpace xent_space(const gqe_xent_args* a, const XentPlan& q, const XentPlan& 
   return s;
 }
 
-hipError_t xent_launch(bool bf16, int dk, int mode, const XentPass& p, hipStream_t s) {
+hipError_t xent_launch(bool bf16, int dk, int mode, bool unit, const XentPass& p, hipStream_t s) {
   switch (dk) {
-    case 64: return bf16 ? gqe_xent_launch_1_64(mode, p, s) : gqe_xent_launch_0_64(mode, p, s);
-    case 128: return bf16 ? gqe_xent_launch_1_128(mode, p, s) : gqe_xent_launch_0_128(mode, p, s);
-    case 192: return bf16 ? gqe_xent_launch_1_192(mode, p, s) : gqe_xent_launch_0_192(mode, p, s);
-    default: return bf16 ? gqe_xent_launch_1_256(mode, p, s) : gqe_xent_launch_0_256(mode, p, s);
+    case 64: return bf16 ? gqe_xent_launch_1_64(mode, unit, p, s) : gqe_xent_launch_0_64(mode, unit, p, s);
+    case 128: return bf16 ? gqe_xent_launch_1_128(mode, unit, p, s) : gqe_xent_launch_0_128(mode, unit, p, s);
+    case 192: return bf16 ? gqe_xent_launch_1_192(mode, unit, p, s) : gqe_xent_launch_0_192(mode, unit, p, s);
+    default: return bf16 ? gqe_xent_launch_1_256(mode, unit, p, s) : gqe_xent_launch_0_256(mode, unit, p, s);
   }
 }
 
@@ -355,9 +355,8 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
   if (first && B) {
     p.y = a->q; p.y_stride = a->q_stride; p.ny = (int32_t)B; p.y_vec = rows_vec(a->q, a->q_stride);
     p.x = a->table; p.x_stride = a->table_stride; p.nx = (int32_t)V; p.x_vec = rows_vec(a->table, a->table_stride);
-    p.x_unit = a->normalize ? 1 : 0;
     p.n_tiles = pq.n_tiles; p.tiles_per_split = pq.per; p.n_split = pq.n_split; p.n_yblk = pq.n_yblk;
-    hipError_t e = xent_launch(bf16, pq.dk, dq ? XENT_MODE_DQ : XENT_MODE_LSE, p, stream);
+    hipError_t e = xent_launch(bf16, pq.dk, dq ? XENT_MODE_DQ : XENT_MODE_LSE, a->normalize != 0, p, stream);
     if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
     j.n_split = pq.n_split; j.ny = (int32_t)B;
     j.loss = a->loss; j.lse = a->lse; j.stat = stat;
@@ -367,13 +366,13 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     if ((e = hipGetLastError()) != hipSuccess) return hip_refuse(e, "softmax_xent");
   }
   if (dt) {
-    p.y = a->table; p.y_stride = a->table_stride; p.ny = (int32_t)V; p.y_vec = rows_vec(a->table, a->table_stride); p.y_unit = a->normalize ? 1 : 0;
-    p.x = a->q; p.x_stride = a->q_stride; p.nx = (int32_t)B; p.x_vec = rows_vec(a->q, a->q_stride); p.x_unit = 0;
+    p.y = a->table; p.y_stride = a->table_stride; p.ny = (int32_t)V; p.y_vec = rows_vec(a->table, a->table_stride);
+    p.x = a->q; p.x_stride = a->q_stride; p.nx = (int32_t)B; p.x_vec = rows_vec(a->q, a->q_stride);
     p.weight = a->weight;
     p.n_tiles = pt.n_tiles; p.tiles_per_split = pt.per; p.n_split = pt.n_split; p.n_yblk = pt.n_yblk;
     p.out = a->dtable; p.out_stride = a->dtable_stride; p.accumulate = a->accumulate;
     p.out_vec = a->dim % 4 == 0 && aligned(a->dtable, bf16 ? 8 : 16) && a->dtable_stride % 4 == 0;
-    hipError_t e = xent_launch(bf16, pt.dk, XENT_MODE_DT, p, stream);
+    hipError_t e = xent_launch(bf16, pt.dk, XENT_MODE_DT, a->normalize != 0, p, stream);
     if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
     if (pt.n_split > 1) {
       j.n_split = pt.n_split; j.ny = (int32_t)V;

@@ -37,8 +37,11 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 
 #define XENT_BM 128            // stationary rows of a workgroup: 32 for each of its four waves
 #define XENT_TR 32             // streamed rows of an LDS tile
-#ifndef XENT_GROUP
-#define XENT_GROUP 4
+#define XENT_GROUP(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
+#ifndef XENT_AHEAD
+#define XENT_AHEAD 8
+#define XENT_VB 3
+#define XENT_VC 4
 #endif
 #define XENT_NONE (-1.0e30f)   // running maximum before the first term (finite: its difference from -inf is -inf)
 
@@ -50,7 +53,6 @@ struct XentPass {
   int64_t y_stride, x_stride;
   int32_t ny, nx, d;
   int32_t y_vec, x_vec;        // rows are 16-byte aligned and d is whole vectors
-  int32_t y_unit, x_unit;      // divide these rows by their length
   float scale2;                // scale * log2(e): multiplies s
   float scale;                 // DT: multiplies the result
   int32_t n_tiles, tiles_per_split, n_split, n_yblk;
@@ -76,28 +78,27 @@ __device__ __forceinline__ int xent_row_scale(float m) {
 }
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
-__device__ __forceinline__ uint32_t xent_pack_bf16(float a, float b) {
-  union { __bf16 h[2]; uint32_t u; } r;
-  r.h[0] = (__bf16)a;
-  r.h[1] = (__bf16)b;
-  return r.u;
-}
-__device__ __forceinline__ uint32_t xent_pack_f16(float a, float b) {
-  union { _Float16 h[2]; uint32_t u; } r;
-  r.h[0] = (_Float16)a;
-  r.h[1] = (_Float16)b;
-  return r.u;
-}
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t xent_pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2)); }
+__device__ __forceinline__ uint32_t xent_pack_f16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2)); }
 // x = hi + lo in fp16, two values at a time.  hi has to be ONE number for both uses: left alone, the compiler fuses the product that
 // made x into the conversion on one side only (a single rounding there, two here), and once in some thousand values lo is then the
-// remainder of another hi.  The empty asm makes the values opaque.
+// remainder of another hi.  The empty asm makes the values opaque; the remainders are mixed-precision multiply-adds, x - 1 * hi.
 __device__ __forceinline__ void xent_split(float a, float b, uint32_t& hi, uint32_t& lo) {
   asm("" : "+v"(a), "+v"(b));
-  union { _Float16 h[2]; uint32_t u; } r;
-  r.u = xent_pack_f16(a, b);
-  asm("" : "+v"(r.u));
-  hi = r.u;
-  lo = xent_pack_f16(a - (float)r.h[0], b - (float)r.h[1]);
+  hi = xent_pack_f16(a, b);
+  float ra, rb;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(hi), "v"(a));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(hi), "v"(b));
+  lo = xent_pack_f16(ra, rb);
+}
+// 1 / sqrt(ss) to an ulp; a row of zeros has length "infinity", a row that is not finite stays so
+__device__ __forceinline__ float xent_rsqrt(float ss) {
+  const float y = __builtin_amdgcn_rsqf(ss);
+  const float z = y * fmaf(-0.5f * ss * y, y, 1.5f);
+  return ss > 0.f ? z : (ss == 0.f ? 0.f : ss);
 }
 
 union XentFrag {
@@ -114,268 +115,241 @@ __device__ __forceinline__ f32x16 xent_mfma(const XentFrag& a, const XentFrag& b
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
 }
 
-// n consecutive elements of a row as float, guarded by the row's end (scalar) or whole (vec)
-template <bool BF16, int N>
-__device__ __forceinline__ void xent_load(const void* base, int64_t row_off, int col, int d, bool row_ok, bool vec, float* v) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = 0.f;
-  if (!row_ok || col >= d) return;
-  if (BF16) {
-    const uint16_t* p = (const uint16_t*)base + row_off + col;
-    if (vec) {
-      static_assert(N == 8 || N == 4, "");
-      uint32_t u[N / 2];
-      if (N == 8) {
-        const uint4 t = *(const uint4*)p;
-        u[0] = t.x; u[1] = t.y; u[N / 2 - 2] = t.z; u[N / 2 - 1] = t.w;
-      } else {
-        const uint2 t = *(const uint2*)p;
-        u[0] = t.x; u[1] = t.y;
-      }
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) { v[2 * i] = bf16_lo(u[i]); v[2 * i + 1] = bf16_hi(u[i]); }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (col + i < d) v[i] = __uint_as_float((uint32_t)p[i] << 16);
-    }
-  } else {
-    const float* p = (const float*)base + row_off + col;
-    if (vec) {
-#pragma unroll
-      for (int i = 0; i < N; i += 4) {
-        const float4 t = *(const float4*)(p + i);
-        v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (col + i < d) v[i] = p[i];
-    }
-  }
-}
+// Rows of a matrix in global memory.
+struct XentRows {
+  const void* p;
+  int64_t stride;
+  int32_t n, d, vec;
+};
+
+// LDS tile: 32 rows of each plane, a row every 256 ceil(DK / 128) bytes, its 16-byte pieces permuted: piece c of row r stands at
+// c ^ f(r) (low four bits), f(r) = 4 (r & 3) + (r >> 2 & 3).  16 rows at one piece (the first product's operand) and 4 rows at 4
+// neighbouring pieces (the transposed reads of the second) then both touch all 64 banks once.
+__device__ __forceinline__ int xent_swizzle(int row) { return (row & 3) << 2 | (row >> 2 & 3); }
 
 template <bool BF16, int DK, int MODE>
 struct XentLds {
   static constexpr int PLANES = BF16 ? 1 : 2;
-  static constexpr int ROW = 2 * DK + 16;               // bytes of a row of one plane
+  static constexpr int ROW = 256 * ((DK + 127) / 128);
   static constexpr int PLANE = XENT_TR * ROW;
   static constexpr int TILE = PLANES * PLANE;
-  char tile[2][TILE];
-  float cs[2][XENT_TR];      // factor of s
-  float lam[2][XENT_TR];     // added to s
-  float inv[2][XENT_TR];     // LSE / DQ: 2^-lambda
-  float sgn[2][XENT_TR];     // DT
-  float lamt[2][XENT_TR];    // DT: exponent of a target's entry
-  int tgt[2][XENT_TR];       // DT
+  static constexpr int TILES = MODE == XENT_MODE_LSE ? 2 : 3;
+  static constexpr int OUT_ROW = 68;                                  // floats of a row of the outputs' turn (64 columns at a time)
+  static constexpr int OUT = MODE == XENT_MODE_LSE ? 0 : 4 * 32 * OUT_ROW * 4;
+  char tile[TILES * TILE > OUT ? TILES * TILE : OUT];
+  float cs[3][XENT_TR];      // factor of s
+  float lam[3][XENT_TR];     // added to s
+  float inv[3][XENT_TR];     // LSE / DQ: 2^-lambda; DT: sign
+  float lamt[3][XENT_TR];    // DT: exponent of a target's entry
+  int tgt[3][XENT_TR];       // DT
+  float rn[XENT_BM];         // DT: 1 / length of the stationary rows, for the end
 };
 
-// One thread's share of a streamed tile between its global loads and its LDS stores: 8 threads per row, DK / 8 elements each.
-template <bool BF16, int DK, int MODE>
+// One thread's share of 32 rows between their global loads and their LDS stores: 8 threads per row, DK / 8 elements each.
+template <bool BF16, int DK, int ROW, int PLANE, bool UNIT>
 struct XentStage {
-  static constexpr int NCH = DK / 64;          // chunks of 8 elements: chunk c of thread t holds columns 64 c + 8 t ..
+  static constexpr int NCH = DK / 64;          // pieces of 8 elements: piece c of thread t holds columns 64 c + 8 t ..
   uint32_t raw[NCH][BF16 ? 4 : 8];
-  float g, lse2, lr;
-  int tg;
 
-  __device__ __forceinline__ void load(const XentPass& p, int tile, int tid) {
-    const int x = tile * XENT_TR + (tid >> 3), t8 = tid & 7;
-    const bool ok = x < p.nx;
-    const int64_t off = (int64_t)x * p.x_stride;
+  __device__ __forceinline__ void load(const XentRows& r, int row, int t8) {
+    const bool ok = row < r.n;
+    const int64_t off = (int64_t)row * r.stride;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = 64 * c + 8 * t8;
+#pragma unroll
+      for (int i = 0; i < (BF16 ? 4 : 8); ++i) raw[c][i] = 0;
+      if (!ok || col >= r.d) continue;
       if (BF16) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (ok && col < p.d) {
-          const uint16_t* q = (const uint16_t*)p.x + off + col;
-          if (p.x_vec) u = *(const uint4*)q;
-          else {
-            uint32_t e[8];
+        const uint16_t* q = (const uint16_t*)r.p + off + col;
+        if (r.vec) {
+          const uint4 u = *(const uint4*)q;
+          raw[c][0] = u.x; raw[c][1] = u.y; raw[c][2] = u.z; raw[c][3] = u.w;
+        } else {
+          uint32_t e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = col + i < p.d ? q[i] : 0;
-            u = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-          }
+          for (int i = 0; i < 8; ++i) e[i] = col + i < r.d ? q[i] : 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) raw[c][i] = e[2 * i] | e[2 * i + 1] << 16;
         }
-        raw[c][0] = u.x; raw[c][1] = u.y; raw[c][2] = u.z; raw[c][3] = u.w;
       } else {
-        float v[8];
-        xent_load<false, 8>(p.x, off, col, p.d, ok, p.x_vec != 0, v);
+        const float* q = (const float*)r.p + off + col;
+        if (r.vec) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) raw[c][i] = __float_as_uint(v[i]);
-      }
-    }
-    if (MODE == XENT_MODE_DT) {
-      g = 0.f; lse2 = 0.f; lr = 0.f; tg = -1;
-      if (ok) {
-        tg = p.target[x];
-        g = p.weight ? p.weight[x] : 1.f;
-        lse2 = p.stat[2 * (int64_t)x];
-        lr = p.stat[2 * (int64_t)x + 1];
-        if (tg < 0 || tg >= p.ny) { g = 0.f; tg = -1; }
+          for (int i = 0; i < 8; i += 4) {
+            const uint4 u = *(const uint4*)(q + i);
+            raw[c][i] = u.x; raw[c][i + 1] = u.y; raw[c][i + 2] = u.z; raw[c][i + 3] = u.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) raw[c][i] = col + i < r.d ? __float_as_uint(q[i]) : 0;
+        }
       }
     }
   }
 
-  __device__ __forceinline__ void store(const XentPass& p, XentLds<BF16, DK, MODE>& lds, int buf, int tile, int tid) {
-    typedef XentLds<BF16, DK, MODE> L;
-    const int row = tid >> 3, t8 = tid & 7;
-    const bool ok = tile * XENT_TR + row < p.nx;
-    char* base = lds.tile[buf] + row * L::ROW;
-    float cs = 1.f, lam = 0.f;
+  // Operands into the tile (at: this thread's place).  cs: operand times cs is the row (the unit row if
+  // UNIT); k: its power of two, where that is all there is (float32); rn: 1 / length.
+  __device__ __forceinline__ void store(char* tile, int at, float& cs, int& k, float& rn) {
+    k = 0;
+    cs = rn = 1.f;
     if (BF16) {
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) *(uint4*)(base + 2 * (64 * c + 8 * t8)) = make_uint4(raw[c][0], raw[c][1], raw[c][2], raw[c][3]);
-      if (p.x_unit) {
-        float mx = 0.f;
+      for (int c = 0; c < NCH; ++c) *(uint4*)(tile + (at ^ 128 * (c & 1)) + 256 * (c >> 1)) = make_uint4(raw[c][0], raw[c][1], raw[c][2], raw[c][3]);
+      if (!UNIT) return;
+    }
+    float mx = 0.f;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
+    for (int c = 0; c < NCH; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(raw[c][i])), fabsf(bf16_hi(raw[c][i]))));
-        mx = fmaxf(mx, __shfl_xor(mx, 1)); mx = fmaxf(mx, __shfl_xor(mx, 2)); mx = fmaxf(mx, __shfl_xor(mx, 4));
-        const float f = xent_pow2(xent_row_scale(mx));
-        float ss = 0.f;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { const float a = bf16_lo(raw[c][i]) * f, b = bf16_hi(raw[c][i]) * f; ss += a * a + b * b; }
-        ss += __shfl_xor(ss, 1); ss += __shfl_xor(ss, 2); ss += __shfl_xor(ss, 4);
-        cs = ss > 0.f ? f / sqrtf(ss) : (ss == 0.f ? 0.f : ss);
-        if (MODE == XENT_MODE_DQ) lam = cs > 0.f ? log2f(cs) : 0.f;
+      for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
+        if (BF16) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(raw[c][i])), fabsf(bf16_hi(raw[c][i]))));
+        else mx = fmaxf(mx, fabsf(__uint_as_float(raw[c][i])));
       }
-    } else {
-      float mx = 0.f;
+    mx = fmaxf(mx, __shfl_xor(mx, 1));
+    mx = fmaxf(mx, __shfl_xor(mx, 2));
+    mx = fmaxf(mx, __shfl_xor(mx, 4));
+    k = xent_row_scale(mx);
+    float f = xent_pow2(k);
+    if (UNIT) {
+      float ss = 0.f;
 #pragma unroll
       for (int c = 0; c < NCH; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(__uint_as_float(raw[c][i])));
-      mx = fmaxf(mx, __shfl_xor(mx, 1)); mx = fmaxf(mx, __shfl_xor(mx, 2)); mx = fmaxf(mx, __shfl_xor(mx, 4));
-      int k = xent_row_scale(mx);
-      float f = xent_pow2(k);
-      if (p.x_unit) {
-        float ss = 0.f;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) { const float a = __uint_as_float(raw[c][i]) * f; raw[c][i] = __float_as_uint(a); ss += a * a; }
-        ss += __shfl_xor(ss, 1); ss += __shfl_xor(ss, 2); ss += __shfl_xor(ss, 4);
-        k = 14;
-        f = ss > 0.f ? 16384.f / sqrtf(ss) : (ss == 0.f ? 0.f : ss);
-      }
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) xent_split(__uint_as_float(raw[c][2 * i]) * f, __uint_as_float(raw[c][2 * i + 1]) * f, hi[i], lo[i]);
-        char* q = base + 2 * (64 * c + 8 * t8);
-        *(uint4*)q = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *(uint4*)(q + L::PLANE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-      cs = xent_pow2(-k);
-      if (MODE != XENT_MODE_LSE) lam = (float)-k;
+        for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
+          if (BF16) {
+            const float a = bf16_lo(raw[c][i]) * f, b = bf16_hi(raw[c][i]) * f;
+            ss += a * a + b * b;
+          } else {
+            const float a = __uint_as_float(raw[c][i]) * f;
+            raw[c][i] = __float_as_uint(a);
+            ss += a * a;
+          }
+        }
+      ss += __shfl_xor(ss, 1);
+      ss += __shfl_xor(ss, 2);
+      ss += __shfl_xor(ss, 4);
+      const float g = xent_rsqrt(ss);
+      rn = g * f;
+      cs = rn;
+      k = 14;
+      f = g * 16384.f;
     }
-    if (t8 == 0) {
-      if (MODE == XENT_MODE_DT) {
-        const float lg = g != 0.f ? log2f(fabsf(g)) : -INFINITY;
-        lds.cs[buf][row] = cs * p.scale2;
-        lds.lam[buf][row] = ok ? lam + (lg - lse2) : -INFINITY;
-        lds.lamt[buf][row] = lam + (lg + lr);
-        lds.sgn[buf][row] = copysignf(1.f, g);
-        lds.tgt[buf][row] = tg;
-      } else {
-        lds.cs[buf][row] = cs;
-        lds.lam[buf][row] = ok ? lam : -INFINITY;
-        lds.inv[buf][row] = BF16 ? exp2f(-lam) : xent_pow2((int)-lam);
-      }
+    if (BF16) return;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xent_split(__uint_as_float(raw[c][2 * i]) * f, __uint_as_float(raw[c][2 * i + 1]) * f, hi[i], lo[i]);
+      char* q = tile + (at ^ 128 * (c & 1)) + 256 * (c >> 1);
+      *(uint4*)q = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *(uint4*)(q + PLANE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
+    cs = xent_pow2(-k);
   }
 };
 
-template <bool BF16, int DK, int MODE>
-__global__ __launch_bounds__(256, DK <= 128 ? 2 : 1) void gqe_xent_kernel(XentPass p) {
+// UNIT: table rows count divided by their length (the streamed rows of LSE / DQ, the stationary ones of DT).
+template <bool BF16, int DK, int MODE, bool UNIT>
+__global__ __launch_bounds__(256, DK <= 128 || (BF16 && DK == 192) ? 2 : 1) void gqe_xent_kernel(XentPass p) {
   typedef XentLds<BF16, DK, MODE> L;
-  extern __shared__ char smem[];
+  typedef XentStage<BF16, DK, L::ROW, L::PLANE, UNIT && MODE != XENT_MODE_DT> Stage;
+  typedef XentStage<BF16, DK, L::ROW, L::PLANE, UNIT && MODE == XENT_MODE_DT> StageY;
+  extern __shared__ __align__(16) char smem[];
   L& lds = *(L*)smem;
   constexpr int PL = BF16 ? 1 : 2, KS = DK / 16, DT = DK / 32;
-  constexpr bool OUT = MODE != XENT_MODE_LSE;
+  constexpr bool OUT = MODE != XENT_MODE_LSE, IS_DT = MODE == XENT_MODE_DT;
   constexpr float TOP = BF16 ? 0.f : 15.f;       // exponentials reach 2^TOP
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, h = lane >> 5;
+  const int srow = tid >> 3, t8 = tid & 7;       // staging: 8 threads per row
   const int split = blockIdx.x % p.n_split, yblk = blockIdx.x / p.n_split;
   const int y0 = yblk * XENT_BM + wave * 32, y = y0 + n;
   const bool active = y0 < p.ny, y_ok = y < p.ny;
   const int tile0 = split * p.tiles_per_split;
   const int tile1 = min(tile0 + p.tiles_per_split, p.n_tiles);
+  const XentRows xr = {p.x, p.x_stride, p.nx, p.d, p.x_vec};
+  const XentRows yr = {p.y, p.y_stride, p.ny, p.d, p.y_vec};
 
-  // stationary rows -> operand registers
+  // this thread's places in a tile (byte offsets; what is added to them later is a multiple of 256, so that other pieces of the row
+  // are one exclusive or away: the bits of the permutation stay put)
+  const int wr = srow * L::ROW + 16 * (t8 ^ xent_swizzle(srow));                        // stage stores; odd pieces of 8 x 8: ^ 128
+  const int rs = n * L::ROW + 16 * (h ^ xent_swizzle(n));                               // first product; k step: ^ 32 k
+  const int orow = 4 * h + ((lane & 15) >> 2);                                         // second product; column tile: ^ 64 i; rows + 8: (+ 8 rows) ^ 32
+  const int ro = orow * L::ROW + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ xent_swizzle(orow)) + 8 * (lane & 1);
+
+  // stationary rows -> operand registers, through LDS 32 rows (a wave's) at a time: whole rows are read, and converted once
   XentFrag yf[PL][KS];
   float cy = 1.f;
   {
-    const int64_t off = (int64_t)y * p.y_stride;
-    if (BF16) {
-      float ss = 0.f, mx = 0.f;
+    StageY st[2];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        float v[8];
-        xent_load<true, 8>(p.y, off, 16 * ks + 8 * h, p.d, y_ok, p.y_vec != 0, v);
+    for (int w = 0; w < 2; ++w) st[w].load(yr, yblk * XENT_BM + 32 * w + srow, t8);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          yf[0][ks].u[i] = __float_as_uint(v[2 * i]) >> 16 | (__float_as_uint(v[2 * i + 1]) & 0xffff0000u);
-          mx = fmaxf(mx, fmaxf(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
-        }
-      }
-      if (MODE == XENT_MODE_DT && p.y_unit) {
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float f = xent_pow2(xent_row_scale(mx));
+    for (int w = 0; w < 4; ++w) {
+      float c, r;
+      int k;
+      st[w & 1].store(lds.tile, wr + (w & 1) * L::TILE, c, k, r);
+      if (w < 2) st[w & 1].load(yr, yblk * XENT_BM + 32 * (w + 2) + srow, t8);
+      if (t8 == 0) { lds.cs[w & 1][srow] = c; lds.rn[32 * w + srow] = r; }
+      __syncthreads();
+      if (wave == w) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { const float a = bf16_lo(yf[0][ks].u[i]) * f, b = bf16_hi(yf[0][ks].u[i]) * f; ss += a * a + b * b; }
-        ss += __shfl_xor(ss, 32);
-        cy = ss > 0.f ? f / sqrtf(ss) : (ss == 0.f ? 0.f : ss);
+          for (int q = 0; q < PL; ++q) *(uint4*)yf[q][ks].u = *(const uint4*)(lds.tile + ((rs + (w & 1) * L::TILE) ^ 32 * (ks & 7)) + 256 * (ks >> 3) + q * L::PLANE);
+        cy = lds.cs[w & 1][n];
       }
-    } else {
-      // the row is read twice (it comes out of the cache the second time): its largest element and length first, then the split,
-      // so that the whole row never sits in registers next to its operands
-      float mx = 0.f, ss = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        float v[8];
-        xent_load<false, 8>(p.y, off, 16 * ks + 8 * h, p.d, y_ok, p.y_vec != 0, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(v[i]));
-      }
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      int k = xent_row_scale(mx);
-      const float f = xent_pow2(k);
-      float f2 = 1.f;
-      if (MODE == XENT_MODE_DT && p.y_unit) {
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          float v[8];
-          xent_load<false, 8>(p.y, off, 16 * ks + 8 * h, p.d, y_ok, p.y_vec != 0, v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) { const float a = v[i] * f; ss += a * a; }
-        }
-        ss += __shfl_xor(ss, 32);
-        k = 14;
-        f2 = ss > 0.f ? 16384.f / sqrtf(ss) : (ss == 0.f ? 0.f : ss);
-      }
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        float v[8];
-        xent_load<false, 8>(p.y, off, 16 * ks + 8 * h, p.d, y_ok, p.y_vec != 0, v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) xent_split(v[2 * i] * f * f2, v[2 * i + 1] * f * f2, yf[0][ks].u[i], yf[PL - 1][ks].u[i]);
-        if (ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-      }
-      cy = xent_pow2(-k);
     }
-    if (MODE != XENT_MODE_DT) cy *= p.scale2;
+    __syncthreads();
+    if (!IS_DT) cy *= p.scale2;
   }
   int tgt = -1;
-  if (MODE != XENT_MODE_DT && y_ok) tgt = p.target[y];
+  if (!IS_DT && y_ok) tgt = p.target[y];
+
+  // streamed rows: loads of tile t + 3 are under way while tile t + 2 is converted and stored, tile t + 1 multiplied, tile t summed
+  Stage stage;
+  float xg = 0.f, xl = 0.f, xs = 0.f;
+  int xt = -1;
+  const auto load = [&](int t) {
+    const int x = t * XENT_TR + srow;
+    stage.load(xr, x, t8);
+    if (IS_DT) {                                 // (all 8 threads of a row: no branch)
+      xg = xl = xs = 0.f;
+      xt = -1;
+      if (x < p.nx) {
+        xt = p.target[x];
+        xg = p.weight ? p.weight[x] : 1.f;
+        xl = p.stat[2 * (int64_t)x];
+        xs = p.stat[2 * (int64_t)x + 1];
+      }
+    }
+  };
+  const auto store = [&](int t, int tb, int ab) {
+    float c, r;
+    int k;
+    stage.store(lds.tile, wr + tb * L::TILE, c, k, r);
+    const bool ok = t * XENT_TR + srow < p.nx;
+    float lam = BF16 ? 0.f : (float)-k, inv = 1.f;
+    if (IS_DT) {
+      const bool counts = xt >= 0 && xt < p.ny;
+      const float lg = counts ? __builtin_amdgcn_logf(fabsf(xg)) : -INFINITY;      // log2; 0 and what is below float32's normal range: no share
+      lds.lamt[ab][srow] = lam + (lg + xs);
+      lds.tgt[ab][srow] = counts ? xt : -1;
+      inv = copysignf(1.f, xg);
+      lam += lg - xl;
+      c *= p.scale2;
+    } else if (MODE == XENT_MODE_LSE) {
+      lam = 0.f;
+    } else if (!BF16) {
+      inv = xent_pow2(k);
+    } else if (UNIT) {
+      lam = c > 0.f ? __builtin_amdgcn_logf(c) : 0.f;
+      inv = __builtin_amdgcn_exp2f(-lam);
+    }
+    lds.cs[ab][srow] = c;
+    lds.lam[ab][srow] = ok ? lam : -INFINITY;
+    lds.inv[ab][srow] = inv;
+  };
 
   float m = XENT_NONE, l = 0.f;
   f32x16 o[OUT ? DT : 1];
@@ -384,71 +358,93 @@ __global__ __launch_bounds__(256, DK <= 128 ? 2 : 1) void gqe_xent_kernel(XentPa
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
 
-  __builtin_amdgcn_sched_barrier(0);
-  XentStage<BF16, DK, MODE> stage;
-  if (tile0 < tile1) {
-    stage.load(p, tile0, tid);
-    stage.store(p, lds, 0, tile0, tid);
-  }
-  __syncthreads();
-  for (int t = tile0; t < tile1; ++t) {
-    const int buf = (t - tile0) & 1;
-    const bool more = t + 1 < tile1;
-    if (more) stage.load(p, t + 1, tid);
-    __builtin_amdgcn_sched_barrier(0);
-    if (active) {
-      const char* xt = lds.tile[buf];
-      // the small products in a sum of their own: every addition rounds at the sum's size, and theirs is 2^-11 of the large one's
-      f32x16 s, sx;
+  f32x16 s;
+  // first product of one tile: S^T = X Y^T.  The small products in a sum of their own, or before the large ones: every addition
+  // rounds at the sum's size, and theirs is 2^-11 of the large one's.  (d <= 128 runs two waves in 512 registers: there one sum, and
+  // the high halves are read twice.)
+  constexpr bool APART = !BF16 && DK > 128;
+  const auto product = [&](int tb) {
+    const int at = rs + tb * L::TILE;
+    f32x16 acc, small;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = sx[r] = 0.f;
+    for (int r = 0; r < 16; ++r) acc[r] = small[r] = 0.f;
+    if (!BF16 && !APART) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         XentFrag a, al;
-        const char* q = xt + n * L::ROW + 2 * (16 * ks + 8 * h);
+        const char* q = lds.tile + (at ^ 32 * (ks & 7)) + 256 * (ks >> 3);
         *(uint4*)a.u = *(const uint4*)q;
-        s = xent_mfma<BF16>(a, yf[0][ks], s);
-        if (!BF16) {
-          *(uint4*)al.u = *(const uint4*)(q + L::PLANE);
-          sx = xent_mfma<BF16>(a, yf[PL - 1][ks], sx);
-          sx = xent_mfma<BF16>(al, yf[0][ks], sx);
-        }
-        if (ks % XENT_GROUP == XENT_GROUP - 1) __builtin_amdgcn_sched_barrier(0);
+        *(uint4*)al.u = *(const uint4*)(q + L::PLANE);
+        acc = xent_mfma<BF16>(a, yf[PL - 1][ks], acc);
+        acc = xent_mfma<BF16>(al, yf[0][ks], acc);
       }
-      if (!BF16) s += sx;
-      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");             // (the high halves are read again, not kept)
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      XentFrag a, al;
+      const char* q = lds.tile + (at ^ 32 * (ks & 7)) + 256 * (ks >> 3);
+      *(uint4*)a.u = *(const uint4*)q;
+      acc = xent_mfma<BF16>(a, yf[0][ks], acc);
+      if (APART) {
+        *(uint4*)al.u = *(const uint4*)(q + L::PLANE);
+        small = xent_mfma<BF16>(a, yf[PL - 1][ks], small);
+        small = xent_mfma<BF16>(al, yf[0][ks], small);
+      }
+    }
+    return APART ? acc + small : acc;
+  };
+
+  if (tile0 < tile1) {
+    load(tile0);
+    store(tile0, 0, 0);
+    if (tile0 + 1 < tile1) {
+      load(tile0 + 1);
+      store(tile0 + 1, 1, 1);
+    }
+    if (tile0 + 2 < tile1) load(tile0 + 2);
+    __syncthreads();
+    if (active) s = product(0);
+    if (!OUT) __syncthreads();                   // two tiles: the first one's place is taken next
+  }
+  int tb = 0, ab = 0;                            // places of tile t: tile modulo TILES, row arrays modulo 3
+  for (int t = tile0; t < tile1; ++t) {
+    const int tb1 = tb + 1 == L::TILES ? 0 : tb + 1, tb2 = tb1 + 1 == L::TILES ? 0 : tb1 + 1;
+    const int ab1 = ab + 1 == 3 ? 0 : ab + 1, ab2 = ab1 + 1 == 3 ? 0 : ab1 + 1;
+    const bool more = t + 1 < tile1;
+    float e[16];
+    unsigned hit = 0;                            // DT: registers that hold a target's own entry (subtracted)
+    if (active) {
       // exponents; register r holds streamed row 8 (r >> 2) + 4 h + (r & 3)
-      float e[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float4 cs = *(const float4*)&lds.cs[buf][8 * q + 4 * h];
-        const float4 la = *(const float4*)&lds.lam[buf][8 * q + 4 * h];
+        const float4 cs = *(const float4*)&lds.cs[ab][8 * q + 4 * h];
+        const float4 la = *(const float4*)&lds.lam[ab][8 * q + 4 * h];
         e[4 * q] = fmaf(s[4 * q], cs.x * cy, la.x);
         e[4 * q + 1] = fmaf(s[4 * q + 1], cs.y * cy, la.y);
         e[4 * q + 2] = fmaf(s[4 * q + 2], cs.z * cy, la.z);
         e[4 * q + 3] = fmaf(s[4 * q + 3], cs.w * cy, la.w);
       }
-      unsigned hit = 0;          // DT: registers that hold a target's own entry (subtracted)
-      if (MODE != XENT_MODE_DT) {
+      if (!IS_DT) {
         const unsigned at = (unsigned)(tgt - t * XENT_TR);
         if (__any(at < XENT_TR)) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int row = 8 * (r >> 2) + 4 * h + (r & 3);
             if ((int)at == row) {
-              p.st[y] = s[r] * (lds.cs[buf][row] * cy);
+              p.st[y] = s[r] * (lds.cs[ab][row] * cy);
               e[r] = -INFINITY;
             }
           }
         }
       } else {
-        const unsigned at = (unsigned)(lds.tgt[buf][n] - y0);
+        const unsigned at = (unsigned)(lds.tgt[ab][n] - y0);
         if (__any(at < 32)) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int row = 8 * (r >> 2) + 4 * h + (r & 3);
-            if (lds.tgt[buf][row] == y) {
-              e[r] = lds.lamt[buf][row];
+            if (lds.tgt[ab][row] == y) {
+              e[r] = lds.lamt[ab][row];
               hit |= 1u << r;
             }
           }
@@ -469,147 +465,194 @@ __global__ __launch_bounds__(256, DK <= 128 ? 2 : 1) void gqe_xent_kernel(XentPa
             for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
         }
       }
+      XentFrag pf[PL][2];
+      const auto exponentials = [&]() {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 iv = *(const float4*)(MODE == XENT_MODE_DT ? &lds.sgn[buf][8 * q + 4 * h] : &lds.inv[buf][8 * q + 4 * h]);
-        const float inv[4] = {iv.x, iv.y, iv.z, iv.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 4 * q + i;
-          e[r] = __builtin_amdgcn_exp2f(e[r] - m);
-          if (MODE == XENT_MODE_DT) e[r] *= inv[i];
-          else l = fmaf(e[r], inv[i], l);
-        }
-      }
-      if (MODE == XENT_MODE_DT && __any(hit != 0)) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) e[r] = hit >> r & 1 ? -e[r] : e[r];
-      }
-      if (OUT) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int sk = 0; sk < 2; ++sk) {
-          XentFrag pf[PL];
+        for (int q = 0; q < 4; ++q) {
+          const float4 iv = *(const float4*)&lds.inv[ab][8 * q + 4 * h];
+          const float inv[4] = {iv.x, iv.y, iv.z, iv.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (BF16) pf[0].u[i] = xent_pack_bf16(e[8 * sk + 2 * i], e[8 * sk + 2 * i + 1]);
-            else xent_split(e[8 * sk + 2 * i], e[8 * sk + 2 * i + 1], pf[0].u[i], pf[PL - 1].u[i]);
+            const int r = 4 * q + i;
+            if (IS_DT) {
+              e[r] = __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f(e[r] - m) * inv[i]) ^ ((hit << (31 - r)) & 0x80000000u));
+            } else {
+              e[r] = __builtin_amdgcn_exp2f(e[r] - m);
+              l = fmaf(e[r], inv[i], l);
+            }
           }
-          // X^T operand: lane's 16-lane group reads 4 rows x 16 columns, transposed
-          const int row = 16 * sk + 4 * h + ((lane & 15) >> 2), col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-          const char* q = xt + row * L::ROW + 2 * col;
-          typedef __attribute__((address_space(3))) s16x4* lp;
+        }
+        if (OUT) {
+#pragma unroll
+          for (int sk = 0; sk < 2; ++sk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (BF16) pf[0][sk].u[i] = xent_pack_bf16(e[8 * sk + 2 * i], e[8 * sk + 2 * i + 1]);
+              else xent_split(e[8 * sk + 2 * i], e[8 * sk + 2 * i + 1], pf[0][sk].u[i], pf[PL - 1][sk].u[i]);
+            }
+        }
+      };
+      if (more) {
+        // next tile's first product, this tile's exponentials in its shadow: operands are read READ_AHEAD products ahead
+        if (DK <= 128 && !BF16) {
+          exponentials();
+          __builtin_amdgcn_sched_barrier(0);
+          s = product(tb1);
+        } else {
+          exponentials();
+          s = product(tb1);
+          XENT_GROUP(0x100, XENT_AHEAD);
+#pragma unroll
+          for (int i = 0; i < (BF16 ? 1 : 3) * KS; ++i) {
+            XENT_GROUP(0x008, 1);
+            XENT_GROUP(0x100, 1);
+            XENT_GROUP(0x002, XENT_VB);
+          }
+        }
+      } else {
+        exponentials();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (OUT) {
+        typedef __attribute__((address_space(3))) s16x4* lp;
+        const int r0 = ro + tb * L::TILE, r1 = (r0 + 8 * L::ROW) ^ 32;
+#pragma unroll
+        for (int sk = 0; sk < 2; ++sk)
 #pragma unroll
           for (int i = 0; i < DT; ++i) {
             XentFrag a, al;
-            a.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 64 * i));
-            a.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 64 * i + 8 * L::ROW));
-            o[i] = xent_mfma<BF16>(a, pf[0], o[i]);
+            const int at = 256 * (i >> 2) + 16 * sk * L::ROW;
+            const char *q0 = lds.tile + (r0 ^ 64 * (i & 3)) + at, *q1 = lds.tile + (r1 ^ 64 * (i & 3)) + at;
+            a.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q0);
+            a.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q1);
+            o[i] = xent_mfma<BF16>(a, pf[0][sk], o[i]);
             if (!BF16) {
-              al.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + L::PLANE + 64 * i));
-              al.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + L::PLANE + 64 * i + 8 * L::ROW));
-              o[i] = xent_mfma<BF16>(a, pf[PL - 1], o[i]);
-              o[i] = xent_mfma<BF16>(al, pf[0], o[i]);
+              al.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q0 + L::PLANE));
+              al.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q1 + L::PLANE));
+              o[i] = xent_mfma<BF16>(a, pf[PL - 1][sk], o[i]);
+              o[i] = xent_mfma<BF16>(al, pf[0][sk], o[i]);
             }
-            if (i % XENT_GROUP == XENT_GROUP - 1) __builtin_amdgcn_sched_barrier(0);
           }
+        // ... and the tile after next is converted and stored in the second product's shadow (behind the last two: nobody reads it)
+        store(t + 2, tb2, ab2);
+        XENT_GROUP(0x100, XENT_AHEAD);
+#pragma unroll
+        for (int i = 0; i < 2 * DT; ++i) {
+          XENT_GROUP(0x008, 1);
+          XENT_GROUP(0x100, 2);
+          XENT_GROUP(0x002, XENT_VC);
+          if (!BF16) {
+            XENT_GROUP(0x008, 1);
+            XENT_GROUP(0x100, 1);
+            XENT_GROUP(0x002, XENT_VC);
+            XENT_GROUP(0x008, 1);
+            XENT_GROUP(0x100, 1);
+            XENT_GROUP(0x002, XENT_VC);
+          }
+          XENT_GROUP(0x200, 1);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
-    if (more) stage.store(p, lds, buf ^ 1, t + 1, tid);
+    if (!OUT || !active) store(t + 2, tb2, ab2);
+    if (t + 3 < tile1) load(t + 3);
     __syncthreads();
+    tb = tb1;
+    ab = ab1;
   }
   if (!active) return;
-  if (MODE != XENT_MODE_DT) l += __shfl_xor(l, 32);
-  if (!y_ok) return;
-  if (MODE != XENT_MODE_DT || p.n_split > 1) {
-    const int64_t at = (int64_t)split * p.ny + y;
-    if (h == 0) {
-      p.part_m[at] = m;
-      if (MODE != XENT_MODE_DT) p.part_l[at] = l;
-    }
-    if (OUT) {
-      float* po = p.part_o + at * p.d;
-      const bool v4 = (p.d & 3) == 0;
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int c = 32 * i + 8 * q + 4 * h;
-          if (v4) {
-            if (c < p.d) *(float4*)(po + c) = make_float4(o[i][4 * q], o[i][4 * q + 1], o[i][4 * q + 2], o[i][4 * q + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (c + j < p.d) po[c + j] = o[i][4 * q + j];
-          }
-        }
-    }
-    return;
+  if (!IS_DT) l += __shfl_xor(l, 32);
+  const int64_t at = (int64_t)split * p.ny + y;
+  const int here = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));      // the lane again: not kept through the loop
+  if (here < 32 && y_ok && (!IS_DT || p.n_split > 1)) {
+    p.part_m[at] = m;
+    if (!IS_DT) p.part_l[at] = l;
   }
-  // DT, every query seen: the gradient of the table's row
-  if (MODE == XENT_MODE_DT) {
+  if (!OUT) return;
+  const bool last = IS_DT && p.n_split == 1;
+  if (last) {
+    // every query seen: the gradient of the table's row.  Through t = w / |w|: (g - t (t . g)) / |w|; t is in the operand
+    // registers, whose halves stand in the other half's order: one exchange between the halves each
     const float half = exp2f(0.5f * m), f = p.scale * half;     // 2^m in two factors: the sums carry the operands' 2^30, 2^m alone may vanish
-    const int64_t off = (int64_t)y * p.y_stride;
-    float along = 0.f, rn2 = 0.f, rn = 1.f;
-    if (p.y_unit) {        // through t = w / |w|: (g - t (t . g)) / |w|
-      // f32: cy undoes the operand's scale 2^14 only, the length is taken from the row again
-      float ss = 0.f;
+    if (UNIT) {
+      const float rn = lds.rn[32 * wave + n];
+      float along = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int q = 0; q < PL; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const auto sw = __builtin_amdgcn_permlane32_swap(yf[q][ks].u[i], yf[q][ks].u[2 + i], false, false);
+            yf[q][ks].u[i] = sw[0];
+            yf[q][ks].u[2 + i] = sw[1];
+          }
+      const auto t_of = [&](int ks, int j) {      // element j of the exchanged operands, unit row
+        if (BF16) return (j & 1 ? bf16_hi(yf[0][ks].u[j >> 1]) : bf16_lo(yf[0][ks].u[j >> 1])) * cy;
+        return ((float)yf[0][ks].h[j] + (float)yf[PL - 1][ks].h[j]) * cy;
+      };
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) along = fmaf(t_of(ks, j), o[ks >> 1][8 * (ks & 1) + j], along);
+      along += __shfl_xor(along, 32);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float v = fmaf(-along, t_of(ks, j), o[ks >> 1][8 * (ks & 1) + j]);
+          o[ks >> 1][8 * (ks & 1) + j] = v * half * f * rn;
+        }
+    } else {
 #pragma unroll
       for (int i = 0; i < DT; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float w[4];
-          xent_load<BF16, 4>(p.y, off, 32 * i + 8 * q + 4 * h, p.d, true, p.y_vec != 0, w);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) { along = fmaf(w[j], o[i][4 * q + j], along); ss = fmaf(w[j], w[j], ss); }
-        }
-      along += __shfl_xor(along, 32);
-      ss += __shfl_xor(ss, 32);
-      rn = ss > 0.f ? 1.f / sqrtf(ss) : (ss == 0.f ? 0.f : ss);
-      rn2 = along * rn * rn;
+        for (int r = 0; r < 16; ++r) o[i][r] *= half * f;
     }
+  }
+  // 64 columns at a time through LDS, so that whole pieces of rows are written
+  float* turn = (float*)lds.tile + wave * 32 * L::OUT_ROW;
+  const int trow = here >> 4, tcol = 4 * (here & 15);
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
+  for (int c = 0; c < DK / 64; ++c) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = 32 * i + 8 * q + 4 * h;
-        float v[4];
-        if (p.y_unit) {
-          float w[4];
-          xent_load<BF16, 4>(p.y, off, c, p.d, true, p.y_vec != 0, w);
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = (o[i][4 * q + j] - w[j] * rn2) * half * f * rn;
-        } else {
+      for (int q = 0; q < 4; ++q)
+        *(float4*)(turn + n * L::OUT_ROW + 32 * i + 8 * q + 4 * h) =
+            make_float4(o[2 * c + i][4 * q], o[2 * c + i][4 * q + 1], o[2 * c + i][4 * q + 2], o[2 * c + i][4 * q + 3]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = o[i][4 * q + j] * half * f;
-        }
-        if (BF16) {
-          uint16_t* po = (uint16_t*)p.out + (int64_t)y * p.out_stride + c;
-          const uint32_t a = xent_pack_bf16(v[0], v[1]), b = xent_pack_bf16(v[2], v[3]);
+    for (int k = 0; k < 8; ++k) {
+      const int row = 4 * k + trow, col = 64 * c + tcol;
+      float4 v = *(const float4*)(turn + row * L::OUT_ROW + tcol);
+      if (y0 + row < p.ny && col < p.d) {
+        if (BF16 && last) {
+          uint16_t* po = (uint16_t*)p.out + (int64_t)(y0 + row) * p.out_stride + col;
+          const uint32_t a = xent_pack_bf16(v.x, v.y), b = xent_pack_bf16(v.z, v.w);
           if (p.out_vec) {
-            if (c < p.d) *(uint2*)po = make_uint2(a, b);
+            *(uint2*)po = make_uint2(a, b);
           } else {
-            const uint16_t e4[4] = {(uint16_t)a, (uint16_t)(a >> 16), (uint16_t)b, (uint16_t)(b >> 16)};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (c + j < p.d) po[j] = e4[j];
+            po[0] = (uint16_t)a;
+            if (col + 1 < p.d) po[1] = (uint16_t)(a >> 16);
+            if (col + 2 < p.d) po[2] = (uint16_t)b;
+            if (col + 3 < p.d) po[3] = (uint16_t)(b >> 16);
           }
         } else {
-          float* po = (float*)p.out + (int64_t)y * p.out_stride + c;
-          if (p.out_vec) {
-            if (c < p.d) {
-              if (p.accumulate) { const float4 w = *(const float4*)po; v[0] += w.x; v[1] += w.y; v[2] += w.z; v[3] += w.w; }
-              *(float4*)po = make_float4(v[0], v[1], v[2], v[3]);
-            }
+          float* po = last ? (float*)p.out + (int64_t)(y0 + row) * p.out_stride + col : p.part_o + ((int64_t)split * p.ny + y0 + row) * p.d + col;
+          if (last ? p.out_vec : (p.d & 3) == 0) {
+            if (last && p.accumulate) { const float4 w = *(const float4*)po; v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w; }
+            *(float4*)po = v;
           } else {
+            const float e4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (c + j < p.d) po[j] = p.accumulate ? po[j] + v[j] : v[j];
+              if (col + j < p.d) po[j] = last && p.accumulate ? po[j] + e4[j] : e4[j];
           }
         }
       }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
