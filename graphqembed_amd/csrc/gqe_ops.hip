@@ -243,8 +243,14 @@ XentPlan xent_plan(int64_t ny, int64_t nx, int dim, int slots) {
 }
 int xent_slots(int dim) { return dim <= 128 ? 512 : 256; }
 
+// Operands are prepared (one more pass over the table: read, written, and read again instead of it) where more than one block of
+// queries would convert the same rows again; up to XENT_BM queries the passes are bound by memory and convert as they go.
+bool xent_prepares(const gqe_xent_args* a) { return a->n_queries > XENT_BM; }
+// bfloat16 rows that are operands as they lie: whole tiles wide, 16-byte pieces
+bool xent_as_is(bool bf16, int dk, int dim, const void* ptr, int64_t stride) { return bf16 && dk == dim && aligned(ptr, 16) && stride % 8 == 0; }
+
 struct XentSpace {
-  int64_t part_m, part_l, st, stat, part_o, total;
+  int64_t part_m, part_l, st, stat, part_o, image[2], fac[2], total;
 };
 XentSpace xent_space(const gqe_xent_args* a, const XentPlan& q, const XentPlan& t) {
   XentSpace s;
@@ -258,16 +264,30 @@ XentSpace xent_space(const gqe_xent_args* a, const XentPlan& q, const XentPlan& 
   s.st = take(first ? 4 * a->n_queries : 0);
   s.stat = take(a->stat ? 0 : 8 * a->n_queries);
   s.part_o = take(4 * (int64_t)a->dim * std::max(dq ? pq : 0, pt));
+  const int64_t n[2] = {a->n_queries, a->n_rows};
+  for (int i = 0; i < 2; ++i) {      // (sizes alone decide: room for the image also where the rows turn out to be usable as they lie)
+    s.image[i] = take(xent_prepares(a) ? up(n[i], XENT_TR) * q.dk * (a->dtype == GQE_BF16 ? 2 : 4) : 0);
+    s.fac[i] = take(xent_prepares(a) ? 8 * n[i] : 0);
+  }
   s.total = at;
   return s;
 }
 
-hipError_t xent_launch(bool bf16, int dk, int mode, bool unit, const XentPass& p, hipStream_t s) {
+hipError_t xent_launch(bool bf16, int dk, int mode, bool unit, bool dma, const XentPass& p, hipStream_t s) {
   switch (dk) {
-    case 64: return bf16 ? gqe_xent_launch_1_64(mode, unit, p, s) : gqe_xent_launch_0_64(mode, unit, p, s);
-    case 128: return bf16 ? gqe_xent_launch_1_128(mode, unit, p, s) : gqe_xent_launch_0_128(mode, unit, p, s);
-    case 192: return bf16 ? gqe_xent_launch_1_192(mode, unit, p, s) : gqe_xent_launch_0_192(mode, unit, p, s);
-    default: return bf16 ? gqe_xent_launch_1_256(mode, unit, p, s) : gqe_xent_launch_0_256(mode, unit, p, s);
+    case 64: return bf16 ? gqe_xent_launch_1_64(mode, unit, dma, p, s) : gqe_xent_launch_0_64(mode, unit, dma, p, s);
+    case 128: return bf16 ? gqe_xent_launch_1_128(mode, unit, dma, p, s) : gqe_xent_launch_0_128(mode, unit, dma, p, s);
+    case 192: return bf16 ? gqe_xent_launch_1_192(mode, unit, dma, p, s) : gqe_xent_launch_0_192(mode, unit, dma, p, s);
+    default: return bf16 ? gqe_xent_launch_1_256(mode, unit, dma, p, s) : gqe_xent_launch_0_256(mode, unit, dma, p, s);
+  }
+}
+
+hipError_t xent_prep(bool bf16, int dk, bool unit, const XentPrep& p, hipStream_t s) {
+  switch (dk) {
+    case 64: return bf16 ? gqe_xent_prep_1_64(unit, p, s) : gqe_xent_prep_0_64(unit, p, s);
+    case 128: return bf16 ? gqe_xent_prep_1_128(unit, p, s) : gqe_xent_prep_0_128(unit, p, s);
+    case 192: return bf16 ? gqe_xent_prep_1_192(unit, p, s) : gqe_xent_prep_0_192(unit, p, s);
+    default: return bf16 ? gqe_xent_prep_1_256(unit, p, s) : gqe_xent_prep_0_256(unit, p, s);
   }
 }
 
@@ -352,11 +372,39 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
   j.part_m = p.part_m; j.part_l = p.part_l; j.part_o = p.part_o; j.st = p.st;
   j.d = a->dim; j.n_rows = (int32_t)V; j.target = a->target; j.weight = a->weight;
   j.table = a->table; j.table_stride = a->table_stride; j.unit = a->normalize ? 1 : 0; j.scale = a->scale;
+  const bool unit = a->normalize != 0, dma = xent_prepares(a);
+  const char* image[2] = {};
+  const float2* fac[2] = {};
+  int64_t stride[2] = {};
+  p.unit = unit;
+  if (dma) {
+    XentPrep r = {};
+    const void* rows[2] = {a->q, a->table};
+    const int64_t n[2] = {B, V}, st[2] = {a->q_stride, a->table_stride};
+    for (int i = 0; i < 2; ++i) {
+      r.r[i] = XentRows{rows[i], st[i], (int32_t)n[i], a->dim, rows_vec(rows[i], st[i])};
+      r.fac[i] = (float2*)(w + sp.fac[i]);
+      r.tiles[i] = (int32_t)((n[i] + XENT_TR - 1) / XENT_TR);
+      fac[i] = r.fac[i];
+      if (xent_as_is(bf16, pq.dk, a->dim, rows[i], st[i])) {
+        image[i] = (const char*)rows[i];
+        stride[i] = st[i];
+      } else {
+        image[i] = r.image[i] = w + sp.image[i];
+      }
+    }
+    const hipError_t e = xent_prep(bf16, pq.dk, unit, r, stream);
+    if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
+  }
   if (first && B) {
     p.y = a->q; p.y_stride = a->q_stride; p.ny = (int32_t)B; p.y_vec = rows_vec(a->q, a->q_stride);
     p.x = a->table; p.x_stride = a->table_stride; p.nx = (int32_t)V; p.x_vec = rows_vec(a->table, a->table_stride);
     p.n_tiles = pq.n_tiles; p.tiles_per_split = pq.per; p.n_split = pq.n_split; p.n_yblk = pq.n_yblk;
-    hipError_t e = xent_launch(bf16, pq.dk, dq ? XENT_MODE_DQ : XENT_MODE_LSE, a->normalize != 0, p, stream);
+    if (dma) {
+      p.y_image = image[0]; p.y_fac = fac[0]; p.y_stride = stride[0];
+      p.x_image = image[1]; p.x_fac = fac[1]; p.x_stride = stride[1];
+    }
+    hipError_t e = xent_launch(bf16, pq.dk, dq ? XENT_MODE_DQ : XENT_MODE_LSE, unit, dma, p, stream);
     if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
     j.n_split = pq.n_split; j.ny = (int32_t)B;
     j.loss = a->loss; j.lse = a->lse; j.stat = stat;
@@ -372,7 +420,11 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     p.n_tiles = pt.n_tiles; p.tiles_per_split = pt.per; p.n_split = pt.n_split; p.n_yblk = pt.n_yblk;
     p.out = a->dtable; p.out_stride = a->dtable_stride; p.accumulate = a->accumulate;
     p.out_vec = a->dim % 4 == 0 && aligned(a->dtable, bf16 ? 8 : 16) && a->dtable_stride % 4 == 0;
-    hipError_t e = xent_launch(bf16, pt.dk, XENT_MODE_DT, a->normalize != 0, p, stream);
+    if (dma) {
+      p.y_image = image[1]; p.y_fac = fac[1]; p.y_stride = stride[1];
+      p.x_image = image[0]; p.x_fac = fac[0]; p.x_stride = stride[0];
+    }
+    hipError_t e = xent_launch(bf16, pt.dk, XENT_MODE_DT, unit, dma, p, stream);
     if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
     if (pt.n_split > 1) {
       j.n_split = pt.n_split; j.ny = (int32_t)V;

@@ -27,6 +27,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "gqe_common.h"
+
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -37,12 +39,28 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 
 #define XENT_BM 128            // stationary rows of a workgroup: 32 for each of its four waves
 #define XENT_TR 32             // streamed rows of an LDS tile
-#define XENT_GROUP(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
-#ifndef XENT_AHEAD
-#define XENT_AHEAD 8
-#define XENT_VB 3
-#define XENT_VC 4
+// closes a step of n matrix instructions: LDS reads first, then matrix instructions with vector work between them
+#ifndef XENT_V
+#define XENT_V 5
 #endif
+#define XENT_GROUP(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
+#define XENT_MIX(n)                                      \
+  do {                                                   \
+    XENT_GROUP(0x100, 4);                                \
+    XENT_GROUP(0x008, 1);                                \
+    XENT_GROUP(0x002, XENT_V);                           \
+    if ((n) > 1) {                                       \
+      XENT_GROUP(0x008, 1);                              \
+      XENT_GROUP(0x002, XENT_V);                         \
+    }                                                    \
+    if ((n) > 2) {                                       \
+      XENT_GROUP(0x008, 1);                              \
+      XENT_GROUP(0x002, XENT_V);                         \
+    }                                                    \
+    __builtin_amdgcn_sched_barrier(0);                   \
+  } while (0)
+// two waves in a SIMD's 512 registers, where the operands and sums of 32 stationary rows leave room
+#define XENT_TWO (DK <= 64 || (DK <= 128 && (BF16 || DMA || MODE == XENT_MODE_LSE)))
 #define XENT_NONE (-1.0e30f)   // running maximum before the first term (finite: its difference from -inf is -inf)
 
 enum { XENT_MODE_LSE = 0, XENT_MODE_DQ = 1, XENT_MODE_DT = 2 };
@@ -53,6 +71,9 @@ struct XentPass {
   int64_t y_stride, x_stride;
   int32_t ny, nx, d;
   int32_t y_vec, x_vec;        // rows are 16-byte aligned and d is whole vectors
+  const char *y_image, *x_image;      // DMA: prepared tiles, or bfloat16 rows (then the strides are not 0)
+  const float2 *y_fac, *x_fac;        // DMA: factors of the rows
+  int32_t unit;                // DMA, DT: table rows count divided by their length
   float scale2;                // scale * log2(e): multiplies s
   float scale;                 // DT: multiplies the result
   int32_t n_tiles, tiles_per_split, n_split, n_yblk;
@@ -122,16 +143,37 @@ struct XentRows {
   int32_t n, d, vec;
 };
 
-// LDS tile: 32 rows of each plane, a row every 256 ceil(DK / 128) bytes, its 16-byte pieces permuted: piece c of row r stands at
-// c ^ f(r) (low four bits), f(r) = 4 (r & 3) + (r >> 2 & 3).  16 rows at one piece (the first product's operand) and 4 rows at 4
-// neighbouring pieces (the transposed reads of the second) then both touch all 64 banks once.
-__device__ __forceinline__ int xent_swizzle(int row) { return (row & 3) << 2 | (row >> 2 & 3); }
+// Tile of operands, in LDS and (where it is prepared once) in memory alike: each plane is sub-tiles of 32 rows x 128 columns (8 KB) and,
+// where DK is 64 or 192, a last one of 32 rows x 64 (4 KB).  A row's 16-byte pieces are permuted so that 16 rows at one piece (the
+// first product's operand) and 4 rows at 4 neighbouring pieces (the transposed reads of the second) both touch all 64 banks once:
+//   full sub-tile: row r, piece c at 256 r + 16 (c ^ f(r)),  f(r) = 4 (r & 3) + (r >> 2 & 3)
+//   half sub-tile: two rows share 256 bytes:  256 (r >> 1) + 16 (8 (r & 1) + (c ^ g(r >> 1))),  g(s) = 4 (s & 1) + (s >> 1 & 3)
+// Neighbouring column groups are an exclusive or away (bits 5 .. 7), further sub-tiles and rows + 16 a constant, rows + 8 a constant
+// and an exclusive or with 32.
+__device__ __forceinline__ int xent_full(int row, int piece) { return 256 * row + 16 * (piece ^ ((row & 3) << 2 | (row >> 2 & 3))); }
+__device__ __forceinline__ int xent_half(int row, int piece) {
+  const int s = row >> 1;
+  return 256 * s + 16 * (8 * (row & 1) + (piece ^ ((s & 1) << 2 | (s >> 1 & 3))));
+}
+template <int DK>
+struct XentTile {
+  static constexpr int FULL = DK / 128;                    // full sub-tiles
+  static constexpr bool HALF = DK % 128 != 0;
+  static constexpr int PLANE = XENT_TR * DK * 2;
+  int full, half;                                          // a thread's place in a full / half sub-tile
+  // chunk: which 64 columns; x: the exclusive or that selects 16 / 32 columns inside them or, in a full sub-tile, the other 64
+  __device__ __forceinline__ int at(int chunk, int x) const {
+    return (chunk >> 1) * 8192 + (chunk >> 1 < FULL ? full ^ (x | (chunk & 1) << 7) : half ^ x);
+  }
+  // the same place of another tile.  (The exclusive ors come after the addition, so that they are not kept in registers for all of
+  // the loop; the addition is of whole kilobytes and leaves their bits alone.)
+  __device__ __forceinline__ XentTile plus(int off) const { return XentTile{full + off, half + off}; }
+};
 
 template <bool BF16, int DK, int MODE>
 struct XentLds {
   static constexpr int PLANES = BF16 ? 1 : 2;
-  static constexpr int ROW = 256 * ((DK + 127) / 128);
-  static constexpr int PLANE = XENT_TR * ROW;
+  static constexpr int PLANE = XentTile<DK>::PLANE;
   static constexpr int TILE = PLANES * PLANE;
   static constexpr int TILES = MODE == XENT_MODE_LSE ? 2 : 3;
   static constexpr int OUT_ROW = 68;                                  // floats of a row of the outputs' turn (64 columns at a time)
@@ -139,15 +181,16 @@ struct XentLds {
   char tile[TILES * TILE > OUT ? TILES * TILE : OUT];
   float cs[3][XENT_TR];      // factor of s
   float lam[3][XENT_TR];     // added to s
-  float inv[3][XENT_TR];     // LSE / DQ: 2^-lambda; DT: sign
+  float inv[3][XENT_TR];     // DQ: 2^-lambda; DT: the sign (an integer, 0 or 1)
   float lamt[3][XENT_TR];    // DT: exponent of a target's entry
   int tgt[3][XENT_TR];       // DT
   float rn[XENT_BM];         // DT: 1 / length of the stationary rows, for the end
 };
 
 // One thread's share of 32 rows between their global loads and their LDS stores: 8 threads per row, DK / 8 elements each.
-template <bool BF16, int DK, int ROW, int PLANE, bool UNIT>
+template <bool BF16, int DK, bool UNIT>
 struct XentStage {
+  static constexpr int PLANE = XentTile<DK>::PLANE;
   static constexpr int NCH = DK / 64;          // pieces of 8 elements: piece c of thread t holds columns 64 c + 8 t ..
   uint32_t raw[NCH][BF16 ? 4 : 8];
 
@@ -188,73 +231,157 @@ struct XentStage {
     }
   }
 
-  // Operands into the tile (at: this thread's place).  cs: operand times cs is the row (the unit row if
-  // UNIT); k: its power of two, where that is all there is (float32); rn: 1 / length.
-  __device__ __forceinline__ void store(char* tile, int at, float& cs, int& k, float& rn) {
-    k = 0;
-    cs = rn = 1.f;
-    if (BF16) {
+  // Operands into the tile (w: this thread's place), in STEPS pieces of work that a caller may put between matrix instructions:
+  // largest element, length, then the split and its stores.  Afterwards: operand times cs is the row (the unit row if UNIT); k its
+  // power of two, where that is all there is (float32); rn: 1 / length.
+  static constexpr int STEPS = DK / 16, HEAD = NCH + 2, PER = (STEPS + STEPS - HEAD - 1) / (STEPS - HEAD);
+  float cs, rn, f, sum;
+  int k;
+  uint32_t hi[4], lo[4];
+
+  __device__ __forceinline__ void step(int j, char* tile, const XentTile<DK>& w) {
+    if (j == 0) {
+      k = 0;
+      cs = rn = 1.f;
+      sum = 0.f;
+      if (BF16) {
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) *(uint4*)(tile + (at ^ 128 * (c & 1)) + 256 * (c >> 1)) = make_uint4(raw[c][0], raw[c][1], raw[c][2], raw[c][3]);
-      if (!UNIT) return;
-    }
-    float mx = 0.f;
+        for (int c = 0; c < NCH; ++c) *(uint4*)(tile + w.at(c, 0)) = make_uint4(raw[c][0], raw[c][1], raw[c][2], raw[c][3]);
+      }
+      if (!BF16 || UNIT) {
+        float mx = 0.f;
 #pragma unroll
-    for (int c = 0; c < NCH; ++c)
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+          for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
+            if (BF16) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(raw[c][i])), fabsf(bf16_hi(raw[c][i]))));
+            else mx = fmaxf(mx, fabsf(__uint_as_float(raw[c][i])));
+          }
+        mx = fmaxf(mx, dpp_get<0xB1, 0xF>(mx));        // the row's 8 threads: swaps in fours, then halves mirrored
+        mx = fmaxf(mx, dpp_get<0x4E, 0xF>(mx));
+        mx = fmaxf(mx, dpp_get<0x141, 0xF>(mx));
+        k = xent_row_scale(mx);
+        f = xent_pow2(k);
+      }
+    } else if (UNIT && j <= NCH) {
+      const int c = j - 1;
 #pragma unroll
       for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
-        if (BF16) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(raw[c][i])), fabsf(bf16_hi(raw[c][i]))));
-        else mx = fmaxf(mx, fabsf(__uint_as_float(raw[c][i])));
-      }
-    mx = fmaxf(mx, __shfl_xor(mx, 1));
-    mx = fmaxf(mx, __shfl_xor(mx, 2));
-    mx = fmaxf(mx, __shfl_xor(mx, 4));
-    k = xent_row_scale(mx);
-    float f = xent_pow2(k);
-    if (UNIT) {
-      float ss = 0.f;
-#pragma unroll
-      for (int c = 0; c < NCH; ++c)
-#pragma unroll
-        for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
-          if (BF16) {
-            const float a = bf16_lo(raw[c][i]) * f, b = bf16_hi(raw[c][i]) * f;
-            ss += a * a + b * b;
-          } else {
-            const float a = __uint_as_float(raw[c][i]) * f;
-            raw[c][i] = __float_as_uint(a);
-            ss += a * a;
-          }
+        if (BF16) {
+          const float a = bf16_lo(raw[c][i]) * f, b = bf16_hi(raw[c][i]) * f;
+          sum = fmaf(a, a, sum);
+          sum = fmaf(b, b, sum);
+        } else {
+          const float a = __uint_as_float(raw[c][i]) * f;
+          raw[c][i] = __float_as_uint(a);
+          sum = fmaf(a, a, sum);
         }
-      ss += __shfl_xor(ss, 1);
-      ss += __shfl_xor(ss, 2);
-      ss += __shfl_xor(ss, 4);
-      const float g = xent_rsqrt(ss);
+      }
+    } else if (UNIT && j == NCH + 1) {
+      sum += dpp_get<0xB1, 0xF>(sum);
+      sum += dpp_get<0x4E, 0xF>(sum);
+      sum += dpp_get<0x141, 0xF>(sum);
+      const float g = xent_rsqrt(sum);
       rn = g * f;
       cs = rn;
       k = 14;
       f = g * 16384.f;
-    }
-    if (BF16) return;
+    } else if (!BF16 && j >= HEAD) {
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xent_split(__uint_as_float(raw[c][2 * i]) * f, __uint_as_float(raw[c][2 * i + 1]) * f, hi[i], lo[i]);
-      char* q = tile + (at ^ 128 * (c & 1)) + 256 * (c >> 1);
-      *(uint4*)q = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *(uint4*)(q + PLANE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      for (int q = (j - HEAD) * PER; q < (j - HEAD + 1) * PER && q < STEPS; ++q) {
+        const int c = q >> 2, i = q & 3;
+        xent_split(__uint_as_float(raw[c][2 * i]) * f, __uint_as_float(raw[c][2 * i + 1]) * f, hi[i], lo[i]);
+        if (i == 3) {
+          char* to = tile + w.at(c, 0);
+          *(uint4*)to = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *(uint4*)(to + PLANE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
     }
-    cs = xent_pow2(-k);
+    if (!BF16 && j == STEPS - 1) cs = xent_pow2(-k);
+  }
+  __device__ __forceinline__ void store(char* tile, const XentTile<DK>& w) {
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) step(j, tile, w);
   }
 };
 
-// UNIT: table rows count divided by their length (the streamed rows of LSE / DQ, the stationary ones of DT).
-template <bool BF16, int DK, int MODE, bool UNIT>
-__global__ __launch_bounds__(256, DK <= 128 || (BF16 && DK == 192) ? 2 : 1) void gqe_xent_kernel(XentPass p) {
+// Operands prepared once: tiles of both matrices in the layout of LDS, and each row's factors {operand -> row, 1 / length}.  IMAGE =
+// false: only the factors (bfloat16 rows are operands as they are).  One workgroup per 32 rows: memory's rate.
+struct XentPrep {
+  XentRows r[2];               // queries, table
+  char* image[2];
+  float2* fac[2];
+  int32_t tiles[2];
+};
+template <bool BF16, int DK, bool UNIT>
+__device__ __forceinline__ void xent_prep(const XentPrep& p, int which, int tile, char* turn) {
+  constexpr int TILE = (BF16 ? 1 : 2) * XentTile<DK>::PLANE;
+  const int row = threadIdx.x >> 3, t8 = threadIdx.x & 7;
+  XentStage<BF16, DK, UNIT> st;
+  st.load(p.r[which], tile * XENT_TR + row, t8);
+  st.store(turn, XentTile<DK>{xent_full(row, t8), xent_half(row, t8)});
+  if (t8 == 0 && tile * XENT_TR + row < p.r[which].n) p.fac[which][tile * XENT_TR + row] = make_float2(st.cs, st.rn);
+  if (!p.image[which]) return;
+  __syncthreads();             // through LDS: the image is written in order
+  uint4* out = (uint4*)(p.image[which] + (int64_t)tile * TILE);
+#pragma unroll
+  for (int i = 0; i < TILE / 4096; ++i) out[i * 256 + threadIdx.x] = ((const uint4*)turn)[i * 256 + threadIdx.x];
+}
+template <bool BF16, int DK, bool UNIT>
+__global__ __launch_bounds__(256) void gqe_xent_prep_kernel(XentPrep p) {
+  __shared__ __align__(16) char turn[(BF16 ? 1 : 2) * XentTile<DK>::PLANE];
+  const int b = blockIdx.x;
+  if (b < p.tiles[0]) xent_prep<BF16, DK, false>(p, 0, b, turn);
+  else xent_prep<BF16, DK, UNIT>(p, 1, b - p.tiles[0], turn);
+}
+
+// Tiles by direct loads into LDS: a wave takes every fourth KB.  Out of an image in order; out of bfloat16 rows (16-byte aligned, d =
+// DK) each lane picks the row and piece that belong at its place, rows behind the last one again (their exponents are -inf).
+template <bool BF16, int DK>
+struct XentDma {
+  static constexpr int TILE = (BF16 ? 1 : 2) * XentTile<DK>::PLANE, N = TILE / 4096;
+  const char* base;
+  int64_t step;                // bytes from tile to tile
+  int64_t stride;              // bytes of a row, 0: image
+  int rows;
+
+  __device__ __forceinline__ void load(int tile, char* lds, int wave, int lane) const {
+    typedef __attribute__((address_space(1))) const void* gp;
+    typedef __attribute__((address_space(3))) void* lp;
+    const char* from = base + (int64_t)tile * step;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = 4096 * i + 1024 * wave;
+      int64_t off = at + 16 * lane;
+      if (BF16 && stride) {
+        const int o = at + 16 * lane, sub = o >> 13, in = o & 8191;
+        int row, piece;
+        if (sub < XentTile<DK>::FULL) {
+          row = in >> 8;
+          piece = 16 * sub + ((in >> 4 & 15) ^ ((row & 3) << 2 | (row >> 2 & 3)));
+        } else {
+          const int s = in >> 8;
+          row = 2 * s + (in >> 7 & 1);
+          piece = 16 * sub + ((in >> 4 & 7) ^ ((s & 1) << 2 | (s >> 1 & 3)));
+        }
+        const int last = rows - 1 - tile * XENT_TR;
+        off = (int64_t)(row < last ? row : last) * stride + 16 * piece;
+      }
+      __builtin_amdgcn_global_load_lds((gp)(from + off), (lp)(lds + at), 16, 0, 0);
+    }
+  }
+};
+
+// UNIT: table rows count divided by their length (the streamed rows of LSE / DQ, the stationary ones of DT).  DMA: operands were prepared
+// (gqe_xent_prep_kernel); else rows are converted here, in the shadow of the second product - right where few queries share a table
+// that would otherwise be read, written and read again.
+template <bool BF16, int DK, int MODE, bool UNIT, bool DMA>
+__global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPass p) {
   typedef XentLds<BF16, DK, MODE> L;
-  typedef XentStage<BF16, DK, L::ROW, L::PLANE, UNIT && MODE != XENT_MODE_DT> Stage;
-  typedef XentStage<BF16, DK, L::ROW, L::PLANE, UNIT && MODE == XENT_MODE_DT> StageY;
+  typedef XentStage<BF16, DK, UNIT && MODE != XENT_MODE_DT> Stage;
+  typedef XentStage<BF16, DK, UNIT && MODE == XENT_MODE_DT> StageY;
+  typedef XentTile<DK> Tile;
   extern __shared__ __align__(16) char smem[];
   L& lds = *(L*)smem;
   constexpr int PL = BF16 ? 1 : 2, KS = DK / 16, DT = DK / 32;
@@ -270,64 +397,91 @@ __global__ __launch_bounds__(256, DK <= 128 || (BF16 && DK == 192) ? 2 : 1) void
   const XentRows xr = {p.x, p.x_stride, p.nx, p.d, p.x_vec};
   const XentRows yr = {p.y, p.y_stride, p.ny, p.d, p.y_vec};
 
-  // this thread's places in a tile (byte offsets; what is added to them later is a multiple of 256, so that other pieces of the row
-  // are one exclusive or away: the bits of the permutation stay put)
-  const int wr = srow * L::ROW + 16 * (t8 ^ xent_swizzle(srow));                        // stage stores; odd pieces of 8 x 8: ^ 128
-  const int rs = n * L::ROW + 16 * (h ^ xent_swizzle(n));                               // first product; k step: ^ 32 k
-  const int orow = 4 * h + ((lane & 15) >> 2);                                         // second product; column tile: ^ 64 i; rows + 8: (+ 8 rows) ^ 32
-  const int ro = orow * L::ROW + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ xent_swizzle(orow)) + 8 * (lane & 1);
+  // this thread's places in a tile
+  const Tile wr = {xent_full(srow, t8), xent_half(srow, t8)};                            // stage stores
+  const Tile rs = {xent_full(n, h), xent_half(n, h)};                                    // first product: row n, half h of 16 columns
+  const int orow = 4 * h + ((lane & 15) >> 2), opiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const Tile ro = {xent_full(orow, opiece) + 8 * (lane & 1), xent_half(orow, opiece) + 8 * (lane & 1)};      // second product, 32 columns
 
-  // stationary rows -> operand registers, through LDS 32 rows (a wave's) at a time: whole rows are read, and converted once
+  // stationary rows -> operand registers, through LDS
   XentFrag yf[PL][KS];
   float cy = 1.f;
-  {
+  const auto take = [&](const char* tile) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int q = 0; q < PL; ++q) *(uint4*)yf[q][ks].u = *(const uint4*)(tile + rs.at(ks >> 2, 32 * (ks & 3)) + q * L::PLANE);
+  };
+  if (DMA) {                                     // two tiles at a time
+    const XentDma<BF16, DK> dy = {p.y_image, p.y_stride ? 64 * p.y_stride : (int64_t)L::TILE, 2 * p.y_stride, p.ny};
+#pragma unroll
+    for (int w = 0; w < 4; w += 2) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (yblk * XENT_BM + 32 * (w + i) < p.ny) dy.load(yblk * (XENT_BM / 32) + w + i, lds.tile + i * L::TILE, wave, lane);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (wave >> 1 == w >> 1) take(lds.tile + (wave & 1) * L::TILE);
+      __syncthreads();
+    }
+    if (y_ok) {
+      const float2 f = p.y_fac[y];
+      cy = f.x;
+      if (IS_DT && h == 0) lds.rn[32 * wave + n] = f.y;
+    }
+  } else {                                       // 32 rows (a wave's) at a time: whole rows are read, and converted once
     StageY st[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) st[w].load(yr, yblk * XENT_BM + 32 * w + srow, t8);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      float c, r;
-      int k;
-      st[w & 1].store(lds.tile, wr + (w & 1) * L::TILE, c, k, r);
+      st[w & 1].store(lds.tile + (w & 1) * L::TILE, wr);
+      const float c = st[w & 1].cs, r = st[w & 1].rn;
       if (w < 2) st[w & 1].load(yr, yblk * XENT_BM + 32 * (w + 2) + srow, t8);
       if (t8 == 0) { lds.cs[w & 1][srow] = c; lds.rn[32 * w + srow] = r; }
       __syncthreads();
       if (wave == w) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int q = 0; q < PL; ++q) *(uint4*)yf[q][ks].u = *(const uint4*)(lds.tile + ((rs + (w & 1) * L::TILE) ^ 32 * (ks & 7)) + 256 * (ks >> 3) + q * L::PLANE);
+        take(lds.tile + (w & 1) * L::TILE);
         cy = lds.cs[w & 1][n];
       }
     }
     __syncthreads();
-    if (!IS_DT) cy *= p.scale2;
   }
+  if (!IS_DT) cy *= p.scale2;
   int tgt = -1;
   if (!IS_DT && y_ok) tgt = p.target[y];
 
-  // streamed rows: loads of tile t + 3 are under way while tile t + 2 is converted and stored, tile t + 1 multiplied, tile t summed
+  // Streamed rows.  DMA: tile t + 2 arrives while tile t + 1 is multiplied and tile t summed; lanes 0 .. 31 of the workgroup bring
+  // its rows' factors.  Otherwise: loads of tile t + 3 are under way while tile t + 2 is converted and stored.
   Stage stage;
+  const XentDma<BF16, DK> dx = {p.x_image, p.x_stride ? 64 * p.x_stride : (int64_t)L::TILE, 2 * p.x_stride, p.nx};
   float xg = 0.f, xl = 0.f, xs = 0.f;
+  float2 xf = make_float2(1.f, 1.f);
   int xt = -1;
-  const auto load = [&](int t) {
-    const int x = t * XENT_TR + srow;
-    stage.load(xr, x, t8);
-    if (IS_DT) {                                 // (all 8 threads of a row: no branch)
+  const int frow = DMA ? tid & 31 : srow;        // whose factors this thread brings
+  const auto load = [&](int t, int tb) {
+    const int x = t * XENT_TR + frow;
+    if (DMA) dx.load(t, lds.tile + tb * L::TILE, wave, lane);
+    else stage.load(xr, x, t8);
+    if (DMA || IS_DT) {
       xg = xl = xs = 0.f;
       xt = -1;
-      if (x < p.nx) {
-        xt = p.target[x];
-        xg = p.weight ? p.weight[x] : 1.f;
-        xl = p.stat[2 * (int64_t)x];
-        xs = p.stat[2 * (int64_t)x + 1];
+      if (x < p.nx && (!DMA || tid < 32)) {
+        if (DMA) xf = p.x_fac[x];
+        if (IS_DT) {
+          xt = p.target[x];
+          xg = p.weight ? p.weight[x] : 1.f;
+          xl = p.stat[2 * (int64_t)x];
+          xs = p.stat[2 * (int64_t)x + 1];
+        }
       }
     }
   };
-  const auto store = [&](int t, int tb, int ab) {
-    float c, r;
-    int k;
-    stage.store(lds.tile, wr + tb * L::TILE, c, k, r);
+  const auto factors = [&](int t, int ab) {       // behind the tile's operands: its rows' factors
+    if (DMA && tid >= 32) return;
+    const int srow = frow;
+    float c = DMA ? xf.x : stage.cs;
+    const int k = DMA ? 127 - (__float_as_int(c) >> 23) : stage.k;      // (float32: c = 2^-k)
     const bool ok = t * XENT_TR + srow < p.nx;
     float lam = BF16 ? 0.f : (float)-k, inv = 1.f;
     if (IS_DT) {
@@ -335,14 +489,14 @@ __global__ __launch_bounds__(256, DK <= 128 || (BF16 && DK == 192) ? 2 : 1) void
       const float lg = counts ? __builtin_amdgcn_logf(fabsf(xg)) : -INFINITY;      // log2; 0 and what is below float32's normal range: no share
       lds.lamt[ab][srow] = lam + (lg + xs);
       lds.tgt[ab][srow] = counts ? xt : -1;
-      inv = copysignf(1.f, xg);
+      inv = __uint_as_float(__float_as_uint(xg) >> 31);
       lam += lg - xl;
       c *= p.scale2;
     } else if (MODE == XENT_MODE_LSE) {
       lam = 0.f;
     } else if (!BF16) {
       inv = xent_pow2(k);
-    } else if (UNIT) {
+    } else if (UNIT || DMA) {                     // (c = 1 where rows count as they are)
       lam = c > 0.f ? __builtin_amdgcn_logf(c) : 0.f;
       inv = __builtin_amdgcn_exp2f(-lam);
     }
@@ -358,76 +512,107 @@ __global__ __launch_bounds__(256, DK <= 128 || (BF16 && DK == 192) ? 2 : 1) void
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
 
-  f32x16 s;
-  // first product of one tile: S^T = X Y^T.  The small products in a sum of their own, or before the large ones: every addition
-  // rounds at the sum's size, and theirs is 2^-11 of the large one's.  (d <= 128 runs two waves in 512 registers: there one sum, and
-  // the high halves are read twice.)
+  // First product of one tile, S^T = X Y^T, a k step at a time; operands are read AHEAD steps before they are used, and `between` is
+  // work for the vector unit in the shadow of each step's matrix instructions (XENT_MIX lays it out).  The small products have a sum of
+  // their own, or go before the large ones: every addition rounds at the sum's size, and theirs is 2^-11 of the large one's.  (d <= 128
+  // runs two waves in 512 registers: there one sum, and the high halves are read twice.)
   constexpr bool APART = !BF16 && DK > 128;
-  const auto product = [&](int tb) {
-    const int at = rs + tb * L::TILE;
+  constexpr int AHEAD = BF16 ? (KS < 6 ? KS : 6) : APART ? 3 : 2;
+  f32x16 s;
+  const auto product = [&](int tb, auto&& between) {
+    const Tile rt = rs.plus(tb * L::TILE);
     f32x16 acc, small;
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = small[r] = 0.f;
+    const auto piece = [&](int ks) { return lds.tile + rt.at(ks >> 2, 32 * (ks & 3)); };
+    XentFrag a[AHEAD + 1], al[AHEAD + 1];
+    const auto fetch = [&](int ks, bool high, bool low) {
+      if (high) *(uint4*)a[ks % (AHEAD + 1)].u = *(const uint4*)piece(ks);
+      if (low) *(uint4*)al[ks % (AHEAD + 1)].u = *(const uint4*)(piece(ks) + L::PLANE);
+    };
     if (!BF16 && !APART) {
 #pragma unroll
+      for (int ks = 0; ks < AHEAD; ++ks) fetch(ks, true, true);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        XentFrag a, al;
-        const char* q = lds.tile + (at ^ 32 * (ks & 7)) + 256 * (ks >> 3);
-        *(uint4*)a.u = *(const uint4*)q;
-        *(uint4*)al.u = *(const uint4*)(q + L::PLANE);
-        acc = xent_mfma<BF16>(a, yf[PL - 1][ks], acc);
-        acc = xent_mfma<BF16>(al, yf[0][ks], acc);
+        if (ks + AHEAD < KS) fetch(ks + AHEAD, true, true);
+        acc = xent_mfma<BF16>(a[ks % (AHEAD + 1)], yf[PL - 1][ks], acc);
+        acc = xent_mfma<BF16>(al[ks % (AHEAD + 1)], yf[0][ks], acc);
+        between(ks);
+        XENT_MIX(2);
       }
       asm volatile("" ::: "memory");             // (the high halves are read again, not kept)
     }
 #pragma unroll
+    for (int ks = 0; ks < AHEAD; ++ks) fetch(ks, true, APART);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      XentFrag a, al;
-      const char* q = lds.tile + (at ^ 32 * (ks & 7)) + 256 * (ks >> 3);
-      *(uint4*)a.u = *(const uint4*)q;
-      acc = xent_mfma<BF16>(a, yf[0][ks], acc);
+      if (ks + AHEAD < KS) fetch(ks + AHEAD, true, APART);
+      acc = xent_mfma<BF16>(a[ks % (AHEAD + 1)], yf[0][ks], acc);
       if (APART) {
-        *(uint4*)al.u = *(const uint4*)(q + L::PLANE);
-        small = xent_mfma<BF16>(a, yf[PL - 1][ks], small);
-        small = xent_mfma<BF16>(al, yf[0][ks], small);
+        small = xent_mfma<BF16>(a[ks % (AHEAD + 1)], yf[PL - 1][ks], small);
+        small = xent_mfma<BF16>(al[ks % (AHEAD + 1)], yf[0][ks], small);
       }
+      if (BF16 || APART) between(ks);
+      XENT_MIX(APART ? 3 : 1);
     }
-    return APART ? acc + small : acc;
+    s = APART ? acc + small : acc;
+  };
+  // exponents of a tile whose s is complete, and their largest; register r holds streamed row 8 (r >> 2) + 4 h + (r & 3)
+  float e[16], top = 0.f;
+  const auto exponents = [&](int q, int ab) {
+    const float4 cs = *(const float4*)&lds.cs[ab][8 * q + 4 * h];
+    const float4 la = *(const float4*)&lds.lam[ab][8 * q + 4 * h];
+    e[4 * q] = fmaf(s[4 * q], cs.x * cy, la.x);
+    e[4 * q + 1] = fmaf(s[4 * q + 1], cs.y * cy, la.y);
+    e[4 * q + 2] = fmaf(s[4 * q + 2], cs.z * cy, la.z);
+    e[4 * q + 3] = fmaf(s[4 * q + 3], cs.w * cy, la.w);
+    const float t4 = fmaxf(fmaxf(e[4 * q], e[4 * q + 1]), fmaxf(e[4 * q + 2], e[4 * q + 3]));
+    top = q ? fmaxf(top, t4) : t4;
   };
 
   if (tile0 < tile1) {
-    load(tile0);
-    store(tile0, 0, 0);
-    if (tile0 + 1 < tile1) {
-      load(tile0 + 1);
-      store(tile0 + 1, 1, 1);
+    if (DMA) {
+      load(tile0, 0);
+      factors(tile0, 0);
+      if (tile0 + 1 < tile1) {
+        load(tile0 + 1, 1);
+        factors(tile0 + 1, 1);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+      load(tile0, 0);
+      stage.store(lds.tile, wr);
+      factors(tile0, 0);
+      if (tile0 + 1 < tile1) {
+        load(tile0 + 1, 0);
+        stage.store(lds.tile + L::TILE, wr);
+        factors(tile0 + 1, 1);
+      }
+      if (tile0 + 2 < tile1) load(tile0 + 2, 0);
     }
-    if (tile0 + 2 < tile1) load(tile0 + 2);
     __syncthreads();
-    if (active) s = product(0);
+    if (active) {
+      product(0, [](int) {});
+#pragma unroll
+      for (int q = 0; q < 4; ++q) exponents(q, 0);
+    }
     if (!OUT) __syncthreads();                   // two tiles: the first one's place is taken next
   }
   int tb = 0, ab = 0;                            // places of tile t: tile modulo TILES, row arrays modulo 3
   for (int t = tile0; t < tile1; ++t) {
     const int tb1 = tb + 1 == L::TILES ? 0 : tb + 1, tb2 = tb1 + 1 == L::TILES ? 0 : tb1 + 1;
     const int ab1 = ab + 1 == 3 ? 0 : ab + 1, ab2 = ab1 + 1 == 3 ? 0 : ab1 + 1;
-    const bool more = t + 1 < tile1;
-    float e[16];
-    unsigned hit = 0;                            // DT: registers that hold a target's own entry (subtracted)
+    unsigned neg = 0;                            // DT: registers whose entry is subtracted: a negative weight, a target's own (or neither: both)
+    if (DMA && t + 2 < tile1) load(t + 2, tb2);
     if (active) {
-      // exponents; register r holds streamed row 8 (r >> 2) + 4 h + (r & 3)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 cs = *(const float4*)&lds.cs[ab][8 * q + 4 * h];
-        const float4 la = *(const float4*)&lds.lam[ab][8 * q + 4 * h];
-        e[4 * q] = fmaf(s[4 * q], cs.x * cy, la.x);
-        e[4 * q + 1] = fmaf(s[4 * q + 1], cs.y * cy, la.y);
-        e[4 * q + 2] = fmaf(s[4 * q + 2], cs.z * cy, la.z);
-        e[4 * q + 3] = fmaf(s[4 * q + 3], cs.w * cy, la.w);
-      }
+      bool found;                                // a target in this tile: its entry is changed, the largest is taken again
       if (!IS_DT) {
         const unsigned at = (unsigned)(tgt - t * XENT_TR);
-        if (__any(at < XENT_TR)) {
+        found = __any(at < XENT_TR);
+        if (found) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int row = 8 * (r >> 2) + 4 * h + (r & 3);
@@ -438,22 +623,29 @@ __global__ __launch_bounds__(256, DK <= 128 || (BF16 && DK == 192) ? 2 : 1) void
           }
         }
       } else {
-        const unsigned at = (unsigned)(lds.tgt[ab][n] - y0);
-        if (__any(at < 32)) {
+        const unsigned below = (unsigned)__ballot(__float_as_int(lds.inv[ab][n]) != 0) >> 4 * h;      // bit 8 q + i: register 4 q + i
+        if (below) neg = (below & 15) | (below >> 4 & 0xf0) | (below >> 8 & 0xf00) | (below >> 12 & 0xf000);
+        found = __any((unsigned)(lds.tgt[ab][n] - y0) < 32u);
+        if (found) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int row = 8 * (r >> 2) + 4 * h + (r & 3);
             if (lds.tgt[ab][row] == y) {
               e[r] = lds.lamt[ab][row];
-              hit |= 1u << r;
+              neg ^= 1u << r;
             }
           }
         }
       }
-      float top = e[0];
+      if (found) {
+        top = e[0];
 #pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, e[r]);
-      top = fmaxf(top, __shfl_xor(top, 32)) - TOP;
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, e[r]);
+      }
+      {
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - TOP;
+      }
       if (__any(top > m)) {
         const float now = fmaxf(top, m), alpha = exp2f(m - now);
         m = now;
@@ -465,97 +657,85 @@ __global__ __launch_bounds__(256, DK <= 128 || (BF16 && DK == 192) ? 2 : 1) void
             for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
         }
       }
+      // the next tile's first product with this tile's exponentials in its shadow
       XentFrag pf[PL][2];
-      const auto exponentials = [&]() {
+      float4 iv[MODE == XENT_MODE_DQ ? 4 : 1];
+      if (MODE == XENT_MODE_DQ) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 iv = *(const float4*)&lds.inv[ab][8 * q + 4 * h];
-          const float inv[4] = {iv.x, iv.y, iv.z, iv.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 4 * q + i;
-            if (IS_DT) {
-              e[r] = __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f(e[r] - m) * inv[i]) ^ ((hit << (31 - r)) & 0x80000000u));
-            } else {
-              e[r] = __builtin_amdgcn_exp2f(e[r] - m);
-              l = fmaf(e[r], inv[i], l);
-            }
-          }
+        for (int q = 0; q < 4; ++q) iv[q] = *(const float4*)&lds.inv[ab][8 * q + 4 * h];
+      }
+      const auto exponential = [&](int r) {
+        e[r] = __builtin_amdgcn_exp2f(e[r] - m);
+        if (IS_DT) {
+          e[r] = __uint_as_float(__float_as_uint(e[r]) ^ ((neg << (31 - r)) & 0x80000000u));
+        } else if (MODE == XENT_MODE_DQ) {
+          const float inv = (r & 3) == 0 ? iv[r >> 2].x : (r & 3) == 1 ? iv[r >> 2].y : (r & 3) == 2 ? iv[r >> 2].z : iv[r >> 2].w;
+          l = fmaf(e[r], inv, l);
+        } else {
+          l += e[r];
         }
-        if (OUT) {
-#pragma unroll
-          for (int sk = 0; sk < 2; ++sk)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (BF16) pf[0][sk].u[i] = xent_pack_bf16(e[8 * sk + 2 * i], e[8 * sk + 2 * i + 1]);
-              else xent_split(e[8 * sk + 2 * i], e[8 * sk + 2 * i + 1], pf[0][sk].u[i], pf[PL - 1][sk].u[i]);
-            }
+        if (OUT && (r & 1)) {
+          if (BF16) pf[0][r >> 3].u[(r & 7) >> 1] = xent_pack_bf16(e[r - 1], e[r]);
+          else xent_split(e[r - 1], e[r], pf[0][r >> 3].u[(r & 7) >> 1], pf[PL - 1][r >> 3].u[(r & 7) >> 1]);
         }
       };
-      if (more) {
-        // next tile's first product, this tile's exponentials in its shadow: operands are read READ_AHEAD products ahead
-        if (DK <= 128 && !BF16) {
-          exponentials();
-          __builtin_amdgcn_sched_barrier(0);
-          s = product(tb1);
-        } else {
-          exponentials();
-          s = product(tb1);
-          XENT_GROUP(0x100, XENT_AHEAD);
+      if (t + 1 < tile1) {
+        product(tb1, [&](int ks) {
 #pragma unroll
-          for (int i = 0; i < (BF16 ? 1 : 3) * KS; ++i) {
-            XENT_GROUP(0x008, 1);
-            XENT_GROUP(0x100, 1);
-            XENT_GROUP(0x002, XENT_VB);
-          }
-        }
+          for (int r = 0; r < 16; ++r)
+            if (r * KS / 16 == ks || (KS > 16 && r == ks)) exponential(r);
+        });
       } else {
-        exponentials();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) exponential(r);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      // second product, out^T += X^T P, with the conversion of the tile after next (behind the last tiles: of nothing, into a place
+      // that nobody reads) and the next tile's exponents in its shadow
       if (OUT) {
         typedef __attribute__((address_space(3))) s16x4* lp;
-        const int r0 = ro + tb * L::TILE, r1 = (r0 + 8 * L::ROW) ^ 32;
-#pragma unroll
-        for (int sk = 0; sk < 2; ++sk)
-#pragma unroll
-          for (int i = 0; i < DT; ++i) {
-            XentFrag a, al;
-            const int at = 256 * (i >> 2) + 16 * sk * L::ROW;
-            const char *q0 = lds.tile + (r0 ^ 64 * (i & 3)) + at, *q1 = lds.tile + (r1 ^ 64 * (i & 3)) + at;
-            a.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q0);
-            a.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q1);
-            o[i] = xent_mfma<BF16>(a, pf[0][sk], o[i]);
-            if (!BF16) {
-              al.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q0 + L::PLANE));
-              al.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q1 + L::PLANE));
-              o[i] = xent_mfma<BF16>(a, pf[PL - 1][sk], o[i]);
-              o[i] = xent_mfma<BF16>(al, pf[0][sk], o[i]);
-            }
-          }
-        // ... and the tile after next is converted and stored in the second product's shadow (behind the last two: nobody reads it)
-        store(t + 2, tb2, ab2);
-        XENT_GROUP(0x100, XENT_AHEAD);
-#pragma unroll
-        for (int i = 0; i < 2 * DT; ++i) {
-          XENT_GROUP(0x008, 1);
-          XENT_GROUP(0x100, 2);
-          XENT_GROUP(0x002, XENT_VC);
+        const Tile rt = ro.plus(tb * L::TILE);
+        constexpr int NS = 2 * DT, AH = BF16 ? (NS < 4 ? NS : 4) : 2;
+        XentFrag a[AH + 1], al[AH + 1];
+        const auto fetch = [&](int j) {
+          const int sk = j / DT, i = j % DT, chunk = i >> 1, rows = (chunk >> 1 < Tile::FULL ? 256 : 128);
+          const int x = 64 * (i & 1) | (rows == 256 ? (chunk & 1) << 7 : 0), from = 8192 * (chunk >> 1) + 16 * sk * rows;
+          const int r0 = rows == 256 ? rt.full : rt.half;
+          const char *q0 = lds.tile + (r0 ^ x) + from, *q1 = lds.tile + ((r0 + 8 * rows) ^ (x | 32)) + from;
+          a[j % (AH + 1)].q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q0);
+          a[j % (AH + 1)].q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q1);
           if (!BF16) {
-            XENT_GROUP(0x008, 1);
-            XENT_GROUP(0x100, 1);
-            XENT_GROUP(0x002, XENT_VC);
-            XENT_GROUP(0x008, 1);
-            XENT_GROUP(0x100, 1);
-            XENT_GROUP(0x002, XENT_VC);
+            al[j % (AH + 1)].q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q0 + L::PLANE));
+            al[j % (AH + 1)].q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q1 + L::PLANE));
           }
-          XENT_GROUP(0x200, 1);
-        }
+        };
+#pragma unroll
+        for (int j = 0; j < AH; ++j) fetch(j);
         __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          const int sk = j / DT, i = j % DT;
+          if (j + AH < NS) fetch(j + AH);
+          o[i] = xent_mfma<BF16>(a[j % (AH + 1)], pf[0][sk], o[i]);
+          if (!BF16) {
+            o[i] = xent_mfma<BF16>(a[j % (AH + 1)], pf[PL - 1][sk], o[i]);
+            o[i] = xent_mfma<BF16>(al[j % (AH + 1)], pf[0][sk], o[i]);
+          }
+          if (!DMA) stage.step(j, lds.tile + tb2 * L::TILE, wr);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q * NS / 4 == j) exponents(q, ab1);
+          XENT_MIX(BF16 ? 1 : 3);
+        }
       }
     }
-    if (!OUT || !active) store(t + 2, tb2, ab2);
-    if (t + 3 < tile1) load(t + 3);
+    if (!DMA && (!OUT || !active)) stage.store(lds.tile + tb2 * L::TILE, wr);
+    if (!OUT && active) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) exponents(q, ab1);
+    }
+    factors(t + 2, ab2);
+    if (!DMA && t + 3 < tile1) load(t + 3, 0);
+    if (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     tb = tb1;
     ab = ab1;
@@ -574,7 +754,7 @@ __global__ __launch_bounds__(256, DK <= 128 || (BF16 && DK == 192) ? 2 : 1) void
     // every query seen: the gradient of the table's row.  Through t = w / |w|: (g - t (t . g)) / |w|; t is in the operand
     // registers, whose halves stand in the other half's order: one exchange between the halves each
     const float half = exp2f(0.5f * m), f = p.scale * half;     // 2^m in two factors: the sums carry the operands' 2^30, 2^m alone may vanish
-    if (UNIT) {
+    if (DMA ? p.unit != 0 : UNIT) {
       const float rn = lds.rn[32 * wave + n];
       float along = 0.f;
 #pragma unroll
