@@ -66,6 +66,9 @@ struct XentJoin {
   int32_t unit, out_f32, accumulate;
   float scale;
   float *loss, *lse, *stat;
+  XentRec* rec;            // LSE / DQ: the queries as streamed rows of the table's gradient, which this call goes on to
+  const float2* fac;
+  float scale2;
   void* out;
   int64_t out_stride;
 };
@@ -95,15 +98,26 @@ __device__ __forceinline__ double wave_sum_f64(double x) {
   for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
   return x;
 }
+// 2^x and log2 x of a 64-bit number to float32's relative (absolute, below 1) precision: whole powers apart, the rest in float32
+__device__ __forceinline__ float exp2_of(double x) {
+  const double n = floor(fmax(x, -1000.0));
+  return ldexpf(exp2f((float)(x - n)), (int)n);
+}
+__device__ __forceinline__ double log2_of(double x) {
+  int e;
+  const double f = frexp(x, &e);
+  return x > 0.0 ? (double)(e - 1) + (double)log2f((float)(f + f)) : x == 0.0 ? -INFINITY : x;
+}
 
-// One workgroup of WAVES waves per stationary row: the splits' sums brought to one unit and added in a fixed order.  What it reads is
-// n_split rows of partial sums; their latency is hidden by the many rows in flight.
+// One workgroup of WAVES waves per stationary row: the splits' sums brought to one unit and added in a fixed order.  Bound by the
+// latency of n_split rows of partial sums: eight waves share them, 16 bytes a lane, eight of them under way (512 rows of 125 x 512
+// bytes, 33 MB: 10 us; four waves, 4 bytes a lane: 27 us).
 template <bool BF16, int MODE, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
   __shared__ float ws[MODE == XENT_MODE_LSE ? 1 : XENT_MAX_SPLIT];
   __shared__ double red[WAVES];
   __shared__ float redf[WAVES];
-  __shared__ float acc[WAVES][256];
+  __shared__ __align__(16) float acc[WAVES + 1][256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t y = blockIdx.x;
   float m = XENT_NONE;
@@ -131,11 +145,11 @@ __global__ __launch_bounds__(64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
     }
     tg = p.target[y];
     const bool has = tg >= 0 && tg < p.n_rows;
-    const double others = (double)m + log2(l);              // -inf where the target is the only row
+    const double others = (double)m + log2_of(l);           // -inf where the target is the only row
     double lse2 = others, lr = 0.0, loss = 0.0;
     if (has) {
       const double diff = others - (double)p.st[y];          // log2 of (sum of the others / the target's term)
-      const double soft = log1p(exp2(-fabs(diff))) * 1.4426950408889634;
+      const double soft = (double)log1pf(exp2_of(-fabs(diff))) * 1.4426950408889634;
       lse2 = fmax(others, (double)p.st[y]) + soft;
       if (diff != diff) lse2 = diff;
       loss = (fmax(diff, 0.0) + soft) * 0.6931471805599453;
@@ -151,10 +165,19 @@ __global__ __launch_bounds__(64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
       p.stat[2 * y] = (float)lse2;
       p.stat[2 * y + 1] = (float)lr;
     }
+    if (p.rec && tid < XENT_TR) {      // (the last row's workgroup: also what fills its tile)
+      const int i = (int)(y % XENT_TR), last = y == p.ny - 1 ? XENT_TR - 1 : i;
+      if (tid >= i && tid <= last) {
+        const bool ok = tid == i;
+        const float c = ok ? p.fac[y].x : 1.f;
+        xent_rec_dt(p.rec[y / XENT_TR], tid, ok, c, BF16 ? 0.f : xent_exponent(c), ok ? tg : -1, ok ? (p.weight ? p.weight[y] : 1.f) : 0.f, (float)lse2,
+                    (float)lr, p.n_rows, p.scale2);
+      }
+    }
     if (MODE == XENT_MODE_LSE) return;
     if (!has) tg = -1;
-    share = (float)exp2(lr);
-    half = f = (float)exp2(0.5 * ((double)m - lse2));
+    share = exp2_of(lr);
+    half = f = exp2_of(0.5 * ((double)m - lse2));
   } else {
     half = exp2f(0.5f * m);
     f = p.scale * half;
@@ -163,27 +186,46 @@ __global__ __launch_bounds__(64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
   __syncthreads();
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   const int64_t step = (int64_t)p.ny * p.d;
-  const float* po = p.part_o + y * p.d + lane;
-#pragma unroll 4
-  for (int s = wave; s < p.n_split; s += WAVES) {
-    const float w = ws[s];
+  const float* po = p.part_o + y * p.d;
+  const bool vec = (p.d & 3) == 0;
+  if (vec) {                   // d <= 128: two splits at a time, 32 lanes each
+    const int two = p.d <= 128 ? 1 : 0, c = 4 * (two ? lane & 31 : lane);
+    const int first = two ? 2 * wave + (lane >> 5) : wave, stride = two ? 2 * WAVES : WAVES;
+    if (c < p.d) {
+#pragma unroll 8
+      for (int s = first; s < p.n_split; s += stride) {
+        const float w = ws[s];
+        const float4 u = *(const float4*)(po + s * step + c);
+        v[0] = fmaf(w, u.x, v[0]); v[1] = fmaf(w, u.y, v[1]); v[2] = fmaf(w, u.z, v[2]); v[3] = fmaf(w, u.w, v[3]);
+      }
+    }
+    if (two) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (lane + 64 * c < p.d) v[c] = fmaf(w, po[s * step + 64 * c], v[c]);
-  }
-  if (WAVES > 1) {
+      for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], 32);
+    }
+    if (c < 256 && lane * 4 == c) *(float4*)&acc[wave][c] = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll 4
+    for (int s = wave; s < p.n_split; s += WAVES) {
+      const float w = ws[s];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (lane + 64 * c < p.d) v[c] = fmaf(w, po[s * step + lane + 64 * c], v[c]);
+    }
 #pragma unroll
     for (int c = 0; c < 4; ++c) acc[wave][lane + 64 * c] = v[c];
-    __syncthreads();
-    if (wave) return;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-#pragma unroll
-      for (int w = 1; w < WAVES; ++w) v[c] += acc[w][lane + 64 * c];
-    }
   }
+  __syncthreads();
+  if (wave) return;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) v[c] = v[c] * half * f;
+  for (int c = 0; c < 4; ++c) {
+    v[c] = 0.f;
+    if (lane + 64 * c < p.d) {
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) v[c] += acc[w][lane + 64 * c];
+    }
+    v[c] = v[c] * half * f;
+  }
   const int64_t row = MODE == XENT_MODE_DT ? y : tg;
   float t[4] = {0.f, 0.f, 0.f, 0.f}, rn = 1.f;
   if (row >= 0 && (MODE == XENT_MODE_DQ || p.unit)) {
@@ -199,8 +241,7 @@ __global__ __launch_bounds__(64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
       float ss = 0.f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) ss = fmaf(t[c] * k, t[c] * k, ss);
-      ss = wave_sum(ss);
-      rn = ss > 0.f ? k / sqrtf(ss) : (ss == 0.f ? 0.f : ss);
+      rn = xent_rsqrt(wave_sum(ss)) * k;
 #pragma unroll
       for (int c = 0; c < 4; ++c) t[c] *= rn;
     }
@@ -229,15 +270,16 @@ struct XentPlan {
   int dk, n_tiles, n_yblk, n_split, per;
 };
 
-// Splits of the streamed axis: enough workgroups to fill the 256 CUs (`slots` of them at once), never more splits than tiles.
-XentPlan xent_plan(int64_t ny, int64_t nx, int dim, int slots) {
+// Splits of the streamed axis: enough workgroups to fill the 256 CUs (`slots` of them at once), `least` tiles in each.  The table's
+// gradient takes four at least: below that the join costs more than a split saves.
+XentPlan xent_plan(int64_t ny, int64_t nx, int dim, int slots, int least) {
   XentPlan r;
   r.dk = dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
   r.n_tiles = (int)((nx + XENT_TR - 1) / XENT_TR);
   r.n_yblk = (int)((ny + XENT_BM - 1) / XENT_BM);
   int64_t s = std::max<int64_t>(1, slots / std::max(r.n_yblk, 1));
   s = std::min<int64_t>(std::min<int64_t>(s, XENT_MAX_SPLIT), std::max(r.n_tiles, 1));
-  r.per = std::max(1, (int)((r.n_tiles + s - 1) / s));
+  r.per = std::max(least, (int)((r.n_tiles + s - 1) / s));
   r.n_split = std::max(1, (r.n_tiles + r.per - 1) / r.per);
   return r;
 }
@@ -247,10 +289,10 @@ int xent_slots(int dim) { return dim <= 128 ? 512 : 256; }
 // queries would convert the same rows again; up to XENT_BM queries the passes are bound by memory and convert as they go.
 bool xent_prepares(const gqe_xent_args* a) { return a->n_queries > XENT_BM; }
 // bfloat16 rows that are operands as they lie: whole tiles wide, 16-byte pieces
-bool xent_as_is(bool bf16, int dk, int dim, const void* ptr, int64_t stride) { return bf16 && dk == dim && aligned(ptr, 16) && stride % 8 == 0; }
+bool xent_as_is(bool bf16, int dk, int dim, const void* ptr, int64_t stride) { return bf16 && dk == dim && aligned(ptr, 16) && stride % 8 == 0 && stride < (1 << 25); }
 
 struct XentSpace {
-  int64_t part_m, part_l, st, stat, part_o, image[2], fac[2], total;
+  int64_t part_m, part_l, st, stat, part_o, image[2], fac[2], rec, total;
 };
 XentSpace xent_space(const gqe_xent_args* a, const XentPlan& q, const XentPlan& t) {
   XentSpace s;
@@ -269,6 +311,7 @@ XentSpace xent_space(const gqe_xent_args* a, const XentPlan& q, const XentPlan& 
     s.image[i] = take(xent_prepares(a) ? up(n[i], XENT_TR) * q.dk * (a->dtype == GQE_BF16 ? 2 : 4) : 0);
     s.fac[i] = take(xent_prepares(a) ? 8 * n[i] : 0);
   }
+  s.rec = take(xent_prepares(a) ? up(std::max(n[0], n[1]), XENT_TR) / XENT_TR * (int64_t)sizeof(XentRec) : 0);
   s.total = at;
   return s;
 }
@@ -294,9 +337,9 @@ hipError_t xent_prep(bool bf16, int dk, bool unit, const XentPrep& p, hipStream_
 template <int MODE>
 void join_launch(bool bf16, const XentJoin& j, hipStream_t s) {
   const dim3 grid((unsigned)j.ny);
-  if (j.n_split > 4) {
-    if (bf16) gqe_xent_join_kernel<true, MODE, 4><<<grid, dim3(256), 0, s>>>(j);
-    else gqe_xent_join_kernel<false, MODE, 4><<<grid, dim3(256), 0, s>>>(j);
+  if (j.n_split > 8) {
+    if (bf16) gqe_xent_join_kernel<true, MODE, 8><<<grid, dim3(512), 0, s>>>(j);
+    else gqe_xent_join_kernel<false, MODE, 8><<<grid, dim3(512), 0, s>>>(j);
   } else {
     if (bf16) gqe_xent_join_kernel<true, MODE, 1><<<grid, dim3(64), 0, s>>>(j);
     else gqe_xent_join_kernel<false, MODE, 1><<<grid, dim3(64), 0, s>>>(j);
@@ -323,8 +366,8 @@ const char* gqe_ops_last_error(void) { return g_ops_error.c_str(); }
 int64_t gqe_softmax_xent_workspace(const gqe_xent_args* a) {
   const int rc = xent_check_sizes(a);
   if (rc) return rc;
-  const XentPlan q = xent_plan(a->n_queries, a->n_rows, a->dim, xent_slots(a->dim));
-  const XentPlan t = xent_plan(a->n_rows, a->n_queries, a->dim, xent_slots(a->dim));
+  const XentPlan q = xent_plan(a->n_queries, a->n_rows, a->dim, xent_slots(a->dim), 1);
+  const XentPlan t = xent_plan(a->n_rows, a->n_queries, a->dim, xent_slots(a->dim), 4);
   return std::max<int64_t>(256, xent_space(a, q, t).total);
 }
 
@@ -345,7 +388,7 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     return refuse(GQE_ERR_ARG, "softmax_xent: a row stride is smaller than dim %d", a->dim);
   if (!aligned(a->q, esize) || !aligned(a->table, esize) || !aligned(a->dq, a->dq_f32 ? 4 : esize) || !aligned(a->dtable, esize))
     return refuse(GQE_ERR_ARG, "softmax_xent: a pointer is not aligned to its element");
-  const XentPlan pq = xent_plan(B, V, a->dim, xent_slots(a->dim)), pt = xent_plan(V, B, a->dim, xent_slots(a->dim));
+  const XentPlan pq = xent_plan(B, V, a->dim, xent_slots(a->dim), 1), pt = xent_plan(V, B, a->dim, xent_slots(a->dim), 4);
   const XentSpace sp = xent_space(a, pq, pt);
   if (a->workspace_bytes < sp.total || (sp.total && (!a->workspace || !aligned(a->workspace, 256))))
     return refuse(GQE_ERR_WORKSPACE, "softmax_xent: needs %lld workspace bytes, 256-byte aligned; got %lld", (long long)sp.total, (long long)a->workspace_bytes);
@@ -393,6 +436,7 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
         image[i] = r.image[i] = w + sp.image[i];
       }
     }
+    r.rec = first ? (XentRec*)(w + sp.rec) : nullptr;
     const hipError_t e = xent_prep(bf16, pq.dk, unit, r, stream);
     if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
   }
@@ -402,13 +446,16 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     p.n_tiles = pq.n_tiles; p.tiles_per_split = pq.per; p.n_split = pq.n_split; p.n_yblk = pq.n_yblk;
     if (dma) {
       p.y_image = image[0]; p.y_fac = fac[0]; p.y_stride = stride[0];
-      p.x_image = image[1]; p.x_fac = fac[1]; p.x_stride = stride[1];
+      p.x_image = image[1]; p.x_rec = (const XentRec*)(w + sp.rec); p.x_stride = stride[1];
     }
     hipError_t e = xent_launch(bf16, pq.dk, dq ? XENT_MODE_DQ : XENT_MODE_LSE, unit, dma, p, stream);
     if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
     j.n_split = pq.n_split; j.ny = (int32_t)B;
     j.loss = a->loss; j.lse = a->lse; j.stat = stat;
     j.out = a->dq; j.out_stride = a->dq_stride; j.out_f32 = a->dq_f32 || !bf16;
+    if (dma && dt) {
+      j.rec = (XentRec*)(w + sp.rec); j.fac = fac[0]; j.scale2 = p.scale2;
+    }
     if (dq) join_launch<XENT_MODE_DQ>(bf16, j, stream);
     else join_launch<XENT_MODE_LSE>(bf16, j, stream);
     if ((e = hipGetLastError()) != hipSuccess) return hip_refuse(e, "softmax_xent");
@@ -422,7 +469,12 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     p.out_vec = a->dim % 4 == 0 && aligned(a->dtable, bf16 ? 8 : 16) && a->dtable_stride % 4 == 0;
     if (dma) {
       p.y_image = image[1]; p.y_fac = fac[1]; p.y_stride = stride[1];
-      p.x_image = image[0]; p.x_fac = fac[0]; p.x_stride = stride[0];
+      p.x_image = image[0]; p.x_rec = (const XentRec*)(w + sp.rec); p.x_stride = stride[0];
+      if (!first) {
+        XentRecs r = {(XentRec*)(w + sp.rec), fac[0], a->target, a->weight, stat, p.scale2, (int32_t)B, (int32_t)V, bf16};
+        const hipError_t e = gqe_xent_recs(r, stream);
+        if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
+      }
     }
     hipError_t e = xent_launch(bf16, pt.dk, XENT_MODE_DT, unit, dma, p, stream);
     if (e != hipSuccess) return hip_refuse(e, "softmax_xent");

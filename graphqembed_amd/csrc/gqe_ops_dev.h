@@ -6,6 +6,8 @@
 
 struct XentPass;
 struct XentPrep;
+struct XentRecs;
+hipError_t gqe_xent_recs(const XentRecs& p, hipStream_t stream);
 #define GQE_XENT_DECL(b, dk) \
   hipError_t gqe_xent_launch_##b##_##dk(int mode, bool unit, bool dma, const XentPass& p, hipStream_t stream); \
   hipError_t gqe_xent_prep_##b##_##dk(bool unit, const XentPrep& p, hipStream_t stream);

@@ -15,7 +15,7 @@
 // x = hi + lo to 22 bits of the row's largest element; a product is hi hi + hi lo + lo hi on the fp16 matrix cores with float32
 // accumulation (the dropped lo lo is below 2^-22), three times the work of one fp16 product where the float32 matrix
 // instructions take sixteen times.  Scales are exact: they re-enter through the factors cs / cy of s and through lambda.  The
-// exponentials are relative to their running maximum, times 2^15, so that the split keeps 22 bits of those that matter.
+// exponentials are relative to their running maximum, times 2^11 to 2^15, so that the split keeps 22 bits of those that matter.
 // bfloat16 operands: one plane, as they are; the exponentials are rounded to bfloat16 (relative error 2^-9, as the output's own).
 //
 // The target's own term is never part of the sums: dq needs p_target - 1, which cancels when the query is answered well, so the
@@ -42,6 +42,9 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 // closes a step of n matrix instructions: LDS reads first, then matrix instructions with vector work between them
 #ifndef XENT_V
 #define XENT_V 5
+#endif
+#ifndef X_DIST
+#define X_DIST 2
 #endif
 #define XENT_GROUP(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
 #define XENT_MIX(n)                                      \
@@ -72,7 +75,8 @@ struct XentPass {
   int32_t ny, nx, d;
   int32_t y_vec, x_vec;        // rows are 16-byte aligned and d is whole vectors
   const char *y_image, *x_image;      // DMA: prepared tiles, or bfloat16 rows (then the strides are not 0)
-  const float2 *y_fac, *x_fac;        // DMA: factors of the rows
+  const float2* y_fac;         // DMA: factors of the stationary rows
+  const struct XentRec* x_rec; // DMA: the streamed rows' part
   int32_t unit;                // DMA, DT: table rows count divided by their length
   float scale2;                // scale * log2(e): multiplies s
   float scale;                 // DT: multiplies the result
@@ -170,20 +174,42 @@ struct XentTile {
   __device__ __forceinline__ XentTile plus(int off) const { return XentTile{full + off, half + off}; }
 };
 
-template <bool BF16, int DK, int MODE>
+// What a streamed row adds to its exponents, per tile of 32 rows: [0] factor of s, [1] lambda, [2] LSE / DQ: 2^-lambda; DT: exponent of a
+// target's entry, [3] DT: the target's row (low 31 bits; 0x7fffffff: none) and the sign of the weight (bit 31).
+struct XentRec {
+  float v[4][XENT_TR];
+};
+struct XentRecs {              // DT: from the queries' factors, statistics and weights
+  XentRec* rec;
+  const float2* fac;
+  const int32_t* target;
+  const float* weight;
+  const float* stat;
+  float scale2;
+  int32_t n, n_rows, bf16;
+};
+__device__ __forceinline__ void xent_rec_dt(XentRec& r, int i, bool ok, float c, float lam, int tg, float g, float lse2, float lr, int n_rows, float scale2) {
+  const bool counts = ok && tg >= 0 && tg < n_rows;
+  const float lg = counts ? __builtin_amdgcn_logf(fabsf(g)) : -INFINITY;      // log2; 0 and what is below float32's normal range: no share
+  r.v[0][i] = c * scale2;
+  r.v[1][i] = ok ? lam + (lg - lse2) : -INFINITY;
+  r.v[2][i] = lam + (lg + lr);
+  r.v[3][i] = __uint_as_float((counts ? (uint32_t)tg : 0x7fffffffu) | (__float_as_uint(g) & 0x80000000u));
+}
+__device__ __forceinline__ float xent_exponent(float c) { return (float)((__float_as_int(c) >> 23) - 127); }      // log2 of a power of two
+
+template <bool BF16, int DK, int MODE, bool DMA>
 struct XentLds {
   static constexpr int PLANES = BF16 ? 1 : 2;
   static constexpr int PLANE = XentTile<DK>::PLANE;
   static constexpr int TILE = PLANES * PLANE;
-  static constexpr int TILES = MODE == XENT_MODE_LSE ? 2 : 3;
+  static constexpr int DIST = DMA ? X_DIST : 2;                       // tile t + DIST is asked for while tile t is summed
+  static constexpr int TILES = (MODE == XENT_MODE_LSE ? 0 : 1) + DIST;
+  static constexpr int RECS = DIST + 1;
   static constexpr int OUT_ROW = 68;                                  // floats of a row of the outputs' turn (64 columns at a time)
   static constexpr int OUT = MODE == XENT_MODE_LSE ? 0 : 4 * 32 * OUT_ROW * 4;
   char tile[TILES * TILE > OUT ? TILES * TILE : OUT];
-  float cs[3][XENT_TR];      // factor of s
-  float lam[3][XENT_TR];     // added to s
-  float inv[3][XENT_TR];     // DQ: 2^-lambda; DT: the sign (an integer, 0 or 1)
-  float lamt[3][XENT_TR];    // DT: exponent of a target's entry
-  int tgt[3][XENT_TR];       // DT
+  XentRec rec[RECS];
   float rn[XENT_BM];         // DT: 1 / length of the stationary rows, for the end
 };
 
@@ -313,6 +339,7 @@ struct XentPrep {
   char* image[2];
   float2* fac[2];
   int32_t tiles[2];
+  XentRec* rec;                // of the table as streamed rows
 };
 template <bool BF16, int DK, bool UNIT>
 __device__ __forceinline__ void xent_prep(const XentPrep& p, int which, int tile, char* turn) {
@@ -321,7 +348,19 @@ __device__ __forceinline__ void xent_prep(const XentPrep& p, int which, int tile
   XentStage<BF16, DK, UNIT> st;
   st.load(p.r[which], tile * XENT_TR + row, t8);
   st.store(turn, XentTile<DK>{xent_full(row, t8), xent_half(row, t8)});
-  if (t8 == 0 && tile * XENT_TR + row < p.r[which].n) p.fac[which][tile * XENT_TR + row] = make_float2(st.cs, st.rn);
+  if (t8 == 0) {
+    const bool ok = tile * XENT_TR + row < p.r[which].n;
+    if (ok) p.fac[which][tile * XENT_TR + row] = make_float2(st.cs, st.rn);
+    if (which == 1 && p.rec) {
+      // float32: the operand's power of two; bfloat16 unit rows: 1 / length
+      const float lam = !BF16 ? xent_exponent(st.cs) : UNIT && st.cs > 0.f ? __builtin_amdgcn_logf(st.cs) : 0.f;
+      XentRec& r = p.rec[tile];
+      r.v[0][row] = st.cs;
+      r.v[1][row] = ok ? lam : -INFINITY;
+      r.v[2][row] = BF16 ? __builtin_amdgcn_exp2f(-lam) : xent_pow2((int)-lam);
+      r.v[3][row] = 0.f;
+    }
+  }
   if (!p.image[which]) return;
   __syncthreads();             // through LDS: the image is written in order
   uint4* out = (uint4*)(p.image[which] + (int64_t)tile * TILE);
@@ -336,6 +375,28 @@ __global__ __launch_bounds__(256) void gqe_xent_prep_kernel(XentPrep p) {
   else xent_prep<BF16, DK, UNIT>(p, 1, b - p.tiles[0], turn);
 }
 
+// 64 pieces of 16 (4) bytes from base + off(lane) into LDS at `to`, in order of lanes.  Written out: through the builtin the compiler has
+// every LDS read wait for every such load that is under way, wherever it goes.  Nobody but the caller waits for these (vmcnt, in order).
+__device__ __forceinline__ void xent_dma16(const char* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void xent_dma4(const char* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ uint32_t xent_lds_addr(const void* p) {      // wave-uniform
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
+}
+
+template <int>
+__global__ __launch_bounds__(256) void gqe_xent_recs_kernel(XentRecs p) {
+  const int x = blockIdx.x * 256 + threadIdx.x;
+  if (x >= (p.n + XENT_TR - 1) / XENT_TR * XENT_TR) return;
+  const bool ok = x < p.n;
+  const float c = ok ? p.fac[x].x : 1.f;
+  xent_rec_dt(p.rec[x / XENT_TR], x % XENT_TR, ok, c, p.bf16 ? 0.f : xent_exponent(c), ok ? p.target[x] : -1, !ok ? 0.f : p.weight ? p.weight[x] : 1.f,
+              ok ? p.stat[2 * (int64_t)x] : 0.f, ok ? p.stat[2 * (int64_t)x + 1] : 0.f, p.n_rows, p.scale2);
+}
+
 // Tiles by direct loads into LDS: a wave takes every fourth KB.  Out of an image in order; out of bfloat16 rows (16-byte aligned, d =
 // DK) each lane picks the row and piece that belong at its place, rows behind the last one again (their exponents are -inf).
 template <bool BF16, int DK>
@@ -346,30 +407,30 @@ struct XentDma {
   int64_t stride;              // bytes of a row, 0: image
   int rows;
 
-  __device__ __forceinline__ void load(int tile, char* lds, int wave, int lane) const {
-    typedef __attribute__((address_space(1))) const void* gp;
-    typedef __attribute__((address_space(3))) void* lp;
+  // piece i of N of this wave's share of a tile
+  __device__ __forceinline__ void piece(int i, int tile, char* lds, int wave, int lane) const {
     const char* from = base + (int64_t)tile * step;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = 4096 * i + 1024 * wave;
-      int64_t off = at + 16 * lane;
-      if (BF16 && stride) {
-        const int o = at + 16 * lane, sub = o >> 13, in = o & 8191;
-        int row, piece;
-        if (sub < XentTile<DK>::FULL) {
-          row = in >> 8;
-          piece = 16 * sub + ((in >> 4 & 15) ^ ((row & 3) << 2 | (row >> 2 & 3)));
-        } else {
-          const int s = in >> 8;
-          row = 2 * s + (in >> 7 & 1);
-          piece = 16 * sub + ((in >> 4 & 7) ^ ((s & 1) << 2 | (s >> 1 & 3)));
-        }
-        const int last = rows - 1 - tile * XENT_TR;
-        off = (int64_t)(row < last ? row : last) * stride + 16 * piece;
+    const uint32_t to = xent_lds_addr(lds + 1024 * wave) + 4096 * i;
+    if (BF16 && stride) {
+      const int o = 4096 * i + 1024 * wave + 16 * lane, sub = o >> 13, in = o & 8191;
+      int row, piece;
+      if (sub < XentTile<DK>::FULL) {
+        row = in >> 8;
+        piece = 16 * sub + ((in >> 4 & 15) ^ ((row & 3) << 2 | (row >> 2 & 3)));
+      } else {
+        const int s = in >> 8;
+        row = 2 * s + (in >> 7 & 1);
+        piece = 16 * sub + ((in >> 4 & 7) ^ ((s & 1) << 2 | (s >> 1 & 3)));
       }
-      __builtin_amdgcn_global_load_lds((gp)(from + off), (lp)(lds + at), 16, 0, 0);
+      const int last = rows - 1 - tile * XENT_TR;
+      xent_dma16(from, (uint32_t)(row < last ? row : last) * (uint32_t)stride + 16 * piece, to);
+    } else {
+      xent_dma16(from + 4096 * i, 1024 * wave + 16 * lane, to);
     }
+  }
+  __device__ __forceinline__ void load(int tile, char* lds, int wave, int lane) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) piece(i, tile, lds, wave, lane);
   }
 };
 
@@ -378,7 +439,7 @@ struct XentDma {
 // that would otherwise be read, written and read again.
 template <bool BF16, int DK, int MODE, bool UNIT, bool DMA>
 __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPass p) {
-  typedef XentLds<BF16, DK, MODE> L;
+  typedef XentLds<BF16, DK, MODE, DMA> L;
   typedef XentStage<BF16, DK, UNIT && MODE != XENT_MODE_DT> Stage;
   typedef XentStage<BF16, DK, UNIT && MODE == XENT_MODE_DT> StageY;
   typedef XentTile<DK> Tile;
@@ -386,7 +447,9 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   L& lds = *(L*)smem;
   constexpr int PL = BF16 ? 1 : 2, KS = DK / 16, DT = DK / 32;
   constexpr bool OUT = MODE != XENT_MODE_LSE, IS_DT = MODE == XENT_MODE_DT;
-  constexpr float TOP = BF16 ? 0.f : 15.f;       // exponentials reach 2^TOP
+  // The running maximum follows only when it has fallen behind by 2^SLACK (new maxima are frequent, large steps are not): exponentials
+  // reach 2^(TOP + SLACK), which is fp16's range where they are split in two of it, and far from float32's where they are bfloat16.
+  constexpr float TOP = BF16 ? 0.f : 11.f, SLACK = BF16 ? 24.f : 4.f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, h = lane >> 5;
   const int srow = tid >> 3, t8 = tid & 7;       // staging: 8 threads per row
   const int split = blockIdx.x % p.n_split, yblk = blockIdx.x / p.n_split;
@@ -438,11 +501,11 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
       st[w & 1].store(lds.tile + (w & 1) * L::TILE, wr);
       const float c = st[w & 1].cs, r = st[w & 1].rn;
       if (w < 2) st[w & 1].load(yr, yblk * XENT_BM + 32 * (w + 2) + srow, t8);
-      if (t8 == 0) { lds.cs[w & 1][srow] = c; lds.rn[32 * w + srow] = r; }
+      if (t8 == 0) { lds.rec[w & 1].v[0][srow] = c; lds.rn[32 * w + srow] = r; }
       __syncthreads();
       if (wave == w) {
         take(lds.tile + (w & 1) * L::TILE);
-        cy = lds.cs[w & 1][n];
+        cy = lds.rec[w & 1].v[0][n];
       }
     }
     __syncthreads();
@@ -451,58 +514,53 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   int tgt = -1;
   if (!IS_DT && y_ok) tgt = p.target[y];
 
-  // Streamed rows.  DMA: tile t + 2 arrives while tile t + 1 is multiplied and tile t summed; lanes 0 .. 31 of the workgroup bring
-  // its rows' factors.  Otherwise: loads of tile t + 3 are under way while tile t + 2 is converted and stored.
+  // Streamed rows.  DMA: tiles t + 2 and t + 3 are under way while tile t + 1 is multiplied and tile t summed; the vector unit has
+  // nothing to do with them.  Otherwise: loads of tile t + 3 are under way while tile t + 2 is converted and stored.
   Stage stage;
   const XentDma<BF16, DK> dx = {p.x_image, p.x_stride ? 64 * p.x_stride : (int64_t)L::TILE, 2 * p.x_stride, p.nx};
+  constexpr int IN_FLIGHT = XentDma<BF16, DK>::N + 1;      // direct loads of a tile, per wave
   float xg = 0.f, xl = 0.f, xs = 0.f;
-  float2 xf = make_float2(1.f, 1.f);
   int xt = -1;
-  const int frow = DMA ? tid & 31 : srow;        // whose factors this thread brings
-  const auto load = [&](int t, int tb) {
-    const int x = t * XENT_TR + frow;
-    if (DMA) dx.load(t, lds.tile + tb * L::TILE, wave, lane);
-    else stage.load(xr, x, t8);
-    if (DMA || IS_DT) {
+  // DMA: piece i of IN_FLIGHT of tile t; the last one is the rows' part: 512 bytes, each half by two waves (all have as many under way)
+  const auto load_piece = [&](int i, int t, int tb, int ab) {
+    if (i < IN_FLIGHT - 1) dx.piece(i, t, lds.tile + tb * L::TILE, wave, lane);
+    else xent_dma4((const char*)(p.x_rec + t), 256 * (wave & 1) + 4 * lane, xent_lds_addr((char*)&lds.rec[ab] + 256 * (wave & 1)));
+  };
+  const auto load = [&](int t, int tb, int ab) {
+    if (DMA) {
+#pragma unroll
+      for (int i = 0; i < IN_FLIGHT; ++i) load_piece(i, t, tb, ab);
+      return;
+    }
+    const int x = t * XENT_TR + srow;
+    stage.load(xr, x, t8);
+    if (IS_DT) {
       xg = xl = xs = 0.f;
       xt = -1;
-      if (x < p.nx && (!DMA || tid < 32)) {
-        if (DMA) xf = p.x_fac[x];
-        if (IS_DT) {
-          xt = p.target[x];
-          xg = p.weight ? p.weight[x] : 1.f;
-          xl = p.stat[2 * (int64_t)x];
-          xs = p.stat[2 * (int64_t)x + 1];
-        }
+      if (x < p.nx) {
+        xt = p.target[x];
+        xg = p.weight ? p.weight[x] : 1.f;
+        xl = p.stat[2 * (int64_t)x];
+        xs = p.stat[2 * (int64_t)x + 1];
       }
     }
   };
-  const auto factors = [&](int t, int ab) {       // behind the tile's operands: its rows' factors
-    if (DMA && tid >= 32) return;
-    const int srow = frow;
-    float c = DMA ? xf.x : stage.cs;
-    const int k = DMA ? 127 - (__float_as_int(c) >> 23) : stage.k;      // (float32: c = 2^-k)
+  // DMA: the next two tiles have arrived; those asked for behind them may be under way.  (Every step asks for one tile, the last ones for
+  // the last tile again, into a place that nobody reads: the count is always the same.)
+  const auto arrived = [&]() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"((L::DIST - 2) * IN_FLIGHT) : "memory"); };
+  const auto factors = [&](int t, int ab) {       // (not DMA) behind the tile's operands: its rows' part
+    const float c = stage.cs;
     const bool ok = t * XENT_TR + srow < p.nx;
-    float lam = BF16 ? 0.f : (float)-k, inv = 1.f;
+    XentRec& r = lds.rec[ab];
+    float lam = BF16 ? 0.f : (float)-stage.k;
     if (IS_DT) {
-      const bool counts = xt >= 0 && xt < p.ny;
-      const float lg = counts ? __builtin_amdgcn_logf(fabsf(xg)) : -INFINITY;      // log2; 0 and what is below float32's normal range: no share
-      lds.lamt[ab][srow] = lam + (lg + xs);
-      lds.tgt[ab][srow] = counts ? xt : -1;
-      inv = __uint_as_float(__float_as_uint(xg) >> 31);
-      lam += lg - xl;
-      c *= p.scale2;
-    } else if (MODE == XENT_MODE_LSE) {
-      lam = 0.f;
-    } else if (!BF16) {
-      inv = xent_pow2(k);
-    } else if (UNIT || DMA) {                     // (c = 1 where rows count as they are)
-      lam = c > 0.f ? __builtin_amdgcn_logf(c) : 0.f;
-      inv = __builtin_amdgcn_exp2f(-lam);
+      xent_rec_dt(r, srow, ok, c, lam, xt, xg, xl, xs, p.ny, p.scale2);
+    } else {
+      if (BF16 && UNIT) lam = c > 0.f ? __builtin_amdgcn_logf(c) : 0.f;
+      r.v[0][srow] = c;
+      r.v[1][srow] = ok ? lam : -INFINITY;
+      r.v[2][srow] = BF16 ? __builtin_amdgcn_exp2f(-lam) : xent_pow2((int)-lam);
     }
-    lds.cs[ab][srow] = c;
-    lds.lam[ab][srow] = ok ? lam : -INFINITY;
-    lds.inv[ab][srow] = inv;
   };
 
   float m = XENT_NONE, l = 0.f;
@@ -519,41 +577,41 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   constexpr bool APART = !BF16 && DK > 128;
   constexpr int AHEAD = BF16 ? (KS < 6 ? KS : 6) : APART ? 3 : 2;
   f32x16 s;
+  XentFrag fa[AHEAD + 1], fl[AHEAD + 1];
+  const auto fetch = [&](const Tile& rt, int ks, bool low) {
+    const char* q = lds.tile + rt.at(ks >> 2, 32 * (ks & 3));
+    *(uint4*)fa[ks % (AHEAD + 1)].u = *(const uint4*)q;
+    if (low) *(uint4*)fl[ks % (AHEAD + 1)].u = *(const uint4*)(q + L::PLANE);
+  };
   const auto product = [&](int tb, auto&& between) {
     const Tile rt = rs.plus(tb * L::TILE);
     f32x16 acc, small;
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = small[r] = 0.f;
-    const auto piece = [&](int ks) { return lds.tile + rt.at(ks >> 2, 32 * (ks & 3)); };
-    XentFrag a[AHEAD + 1], al[AHEAD + 1];
-    const auto fetch = [&](int ks, bool high, bool low) {
-      if (high) *(uint4*)a[ks % (AHEAD + 1)].u = *(const uint4*)piece(ks);
-      if (low) *(uint4*)al[ks % (AHEAD + 1)].u = *(const uint4*)(piece(ks) + L::PLANE);
-    };
+#pragma unroll
+    for (int ks = 0; ks < AHEAD; ++ks) fetch(rt, ks, !BF16);
+    __builtin_amdgcn_sched_barrier(0);
     if (!BF16 && !APART) {
 #pragma unroll
-      for (int ks = 0; ks < AHEAD; ++ks) fetch(ks, true, true);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        if (ks + AHEAD < KS) fetch(ks + AHEAD, true, true);
-        acc = xent_mfma<BF16>(a[ks % (AHEAD + 1)], yf[PL - 1][ks], acc);
-        acc = xent_mfma<BF16>(al[ks % (AHEAD + 1)], yf[0][ks], acc);
+        if (ks + AHEAD < KS) fetch(rt, ks + AHEAD, true);
+        acc = xent_mfma<BF16>(fa[ks % (AHEAD + 1)], yf[PL - 1][ks], acc);
+        acc = xent_mfma<BF16>(fl[ks % (AHEAD + 1)], yf[0][ks], acc);
         between(ks);
         XENT_MIX(2);
       }
       asm volatile("" ::: "memory");             // (the high halves are read again, not kept)
+#pragma unroll
+      for (int ks = 0; ks < AHEAD; ++ks) fetch(rt, ks, false);
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int ks = 0; ks < AHEAD; ++ks) fetch(ks, true, APART);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      if (ks + AHEAD < KS) fetch(ks + AHEAD, true, APART);
-      acc = xent_mfma<BF16>(a[ks % (AHEAD + 1)], yf[0][ks], acc);
+      if (ks + AHEAD < KS) fetch(rt, ks + AHEAD, APART);
+      acc = xent_mfma<BF16>(fa[ks % (AHEAD + 1)], yf[0][ks], acc);
       if (APART) {
-        small = xent_mfma<BF16>(a[ks % (AHEAD + 1)], yf[PL - 1][ks], small);
-        small = xent_mfma<BF16>(al[ks % (AHEAD + 1)], yf[0][ks], small);
+        small = xent_mfma<BF16>(fa[ks % (AHEAD + 1)], yf[PL - 1][ks], small);
+        small = xent_mfma<BF16>(fl[ks % (AHEAD + 1)], yf[0][ks], small);
       }
       if (BF16 || APART) between(ks);
       XENT_MIX(APART ? 3 : 1);
@@ -563,8 +621,8 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   // exponents of a tile whose s is complete, and their largest; register r holds streamed row 8 (r >> 2) + 4 h + (r & 3)
   float e[16], top = 0.f;
   const auto exponents = [&](int q, int ab) {
-    const float4 cs = *(const float4*)&lds.cs[ab][8 * q + 4 * h];
-    const float4 la = *(const float4*)&lds.lam[ab][8 * q + 4 * h];
+    const float4 cs = *(const float4*)&lds.rec[ab].v[0][8 * q + 4 * h];
+    const float4 la = *(const float4*)&lds.rec[ab].v[1][8 * q + 4 * h];
     e[4 * q] = fmaf(s[4 * q], cs.x * cy, la.x);
     e[4 * q + 1] = fmaf(s[4 * q + 1], cs.y * cy, la.y);
     e[4 * q + 2] = fmaf(s[4 * q + 2], cs.z * cy, la.z);
@@ -575,23 +633,20 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
 
   if (tile0 < tile1) {
     if (DMA) {
-      load(tile0, 0);
-      factors(tile0, 0);
-      if (tile0 + 1 < tile1) {
-        load(tile0 + 1, 1);
-        factors(tile0 + 1, 1);
-      }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < L::DIST; ++i)
+        load(min(tile0 + i, tile1 - 1), i, i);
+      arrived();
     } else {
-      load(tile0, 0);
+      load(tile0, 0, 0);
       stage.store(lds.tile, wr);
       factors(tile0, 0);
       if (tile0 + 1 < tile1) {
-        load(tile0 + 1, 0);
+        load(tile0 + 1, 0, 0);
         stage.store(lds.tile + L::TILE, wr);
         factors(tile0 + 1, 1);
       }
-      if (tile0 + 2 < tile1) load(tile0 + 2, 0);
+      if (tile0 + 2 < tile1) load(tile0 + 2, 0, 0);
     }
     __syncthreads();
     if (active) {
@@ -599,14 +654,19 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
 #pragma unroll
       for (int q = 0; q < 4; ++q) exponents(q, 0);
     }
-    if (!OUT) __syncthreads();                   // two tiles: the first one's place is taken next
+    if (!OUT && !DMA) __syncthreads();           // two tiles: the first one's place is taken next
   }
-  int tb = 0, ab = 0;                            // places of tile t: tile modulo TILES, row arrays modulo 3
+  int mark = 0x7fffffff;                         // DT: target and sign of the next tile's row n
+  if (IS_DT && tile0 < tile1) mark = __float_as_int(lds.rec[0].v[3][n]);
+  int tb = 0, ab = 0;                            // places of tile t: tile modulo TILES, its rows' part modulo RECS
   for (int t = tile0; t < tile1; ++t) {
     const int tb1 = tb + 1 == L::TILES ? 0 : tb + 1, tb2 = tb1 + 1 == L::TILES ? 0 : tb1 + 1;
-    const int ab1 = ab + 1 == 3 ? 0 : ab + 1, ab2 = ab1 + 1 == 3 ? 0 : ab1 + 1;
+    const int ab1 = ab + 1 == L::RECS ? 0 : ab + 1, ab2 = ab1 + 1 == L::RECS ? 0 : ab1 + 1;
     unsigned neg = 0;                            // DT: registers whose entry is subtracted: a negative weight, a target's own (or neither: both)
-    if (DMA && t + 2 < tile1) load(t + 2, tb2);
+    const bool more = t + 1 < tile1;
+    // DMA: tile t + DIST goes into the place before tile t's, last read by the step before this one (LSE: into tile t's own, its product
+    // is done).  Asked for in one go: spread over the steps of the first product it took 4 % longer.
+    if (DMA && more) load(min(t + L::DIST, tile1 - 1), OUT ? (tb == 0 ? L::TILES - 1 : tb - 1) : tb, ab == 0 ? L::RECS - 1 : ab - 1);
     if (active) {
       bool found;                                // a target in this tile: its entry is changed, the largest is taken again
       if (!IS_DT) {
@@ -617,21 +677,21 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
           for (int r = 0; r < 16; ++r) {
             const int row = 8 * (r >> 2) + 4 * h + (r & 3);
             if ((int)at == row) {
-              p.st[y] = s[r] * (lds.cs[ab][row] * cy);
+              p.st[y] = s[r] * (lds.rec[ab].v[0][row] * cy);
               e[r] = -INFINITY;
             }
           }
         }
       } else {
-        const unsigned below = (unsigned)__ballot(__float_as_int(lds.inv[ab][n]) != 0) >> 4 * h;      // bit 8 q + i: register 4 q + i
+        const unsigned below = (unsigned)__ballot(mark < 0) >> 4 * h;      // bit 8 q + i: register 4 q + i
         if (below) neg = (below & 15) | (below >> 4 & 0xf0) | (below >> 8 & 0xf00) | (below >> 12 & 0xf000);
-        found = __any((unsigned)(lds.tgt[ab][n] - y0) < 32u);
+        found = __any((unsigned)((mark & 0x7fffffff) - y0) < 32u);
         if (found) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int row = 8 * (r >> 2) + 4 * h + (r & 3);
-            if (lds.tgt[ab][row] == y) {
-              e[r] = lds.lamt[ab][row];
+            if ((__float_as_int(lds.rec[ab].v[3][row]) & 0x7fffffff) == y) {
+              e[r] = lds.rec[ab].v[2][row];
               neg ^= 1u << r;
             }
           }
@@ -646,7 +706,8 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
         top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - TOP;
       }
-      if (__any(top > m)) {
+      // (a tile with a target: at once, so that a row's largest entry, its own target's, is 1 and rounds to itself)
+      if (__any(top > m + (IS_DT && found ? 0.f : SLACK))) {
         const float now = fmaxf(top, m), alpha = exp2f(m - now);
         m = now;
         l *= alpha;
@@ -659,71 +720,72 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
       }
       // the next tile's first product with this tile's exponentials in its shadow
       XentFrag pf[PL][2];
-      float4 iv[MODE == XENT_MODE_DQ ? 4 : 1];
-      if (MODE == XENT_MODE_DQ) {
+      float4 iv[IS_DT ? 1 : 4];
+      if (!IS_DT) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) iv[q] = *(const float4*)&lds.inv[ab][8 * q + 4 * h];
+        for (int q = 0; q < 4; ++q) iv[q] = *(const float4*)&lds.rec[ab].v[2][8 * q + 4 * h];
       }
       const auto exponential = [&](int r) {
         e[r] = __builtin_amdgcn_exp2f(e[r] - m);
         if (IS_DT) {
           e[r] = __uint_as_float(__float_as_uint(e[r]) ^ ((neg << (31 - r)) & 0x80000000u));
-        } else if (MODE == XENT_MODE_DQ) {
+        } else {
           const float inv = (r & 3) == 0 ? iv[r >> 2].x : (r & 3) == 1 ? iv[r >> 2].y : (r & 3) == 2 ? iv[r >> 2].z : iv[r >> 2].w;
           l = fmaf(e[r], inv, l);
-        } else {
-          l += e[r];
         }
         if (OUT && (r & 1)) {
           if (BF16) pf[0][r >> 3].u[(r & 7) >> 1] = xent_pack_bf16(e[r - 1], e[r]);
           else xent_split(e[r - 1], e[r], pf[0][r >> 3].u[(r & 7) >> 1], pf[PL - 1][r >> 3].u[(r & 7) >> 1]);
         }
       };
-      if (t + 1 < tile1) {
+      typedef __attribute__((address_space(3))) s16x4* lp;
+      const Tile rt2 = ro.plus(tb * L::TILE);
+      constexpr int NS = 2 * DT, AH = BF16 ? (NS < 4 ? NS : 4) : 2;
+      XentFrag oa[OUT ? AH + 1 : 1], ol[OUT ? AH + 1 : 1];
+      const auto fetch2 = [&](int j) {
+        const int sk = j / DT, i = j % DT, chunk = i >> 1, rows = (chunk >> 1 < Tile::FULL ? 256 : 128);
+        const int x = 64 * (i & 1) | (rows == 256 ? (chunk & 1) << 7 : 0), from = 8192 * (chunk >> 1) + 16 * sk * rows;
+        const int r0 = rows == 256 ? rt2.full : rt2.half;
+        const char *q0 = lds.tile + (r0 ^ x) + from, *q1 = lds.tile + ((r0 + 8 * rows) ^ (x | 32)) + from;
+        oa[j % (AH + 1)].q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q0);
+        oa[j % (AH + 1)].q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q1);
+        if (!BF16) {
+          ol[j % (AH + 1)].q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q0 + L::PLANE));
+          ol[j % (AH + 1)].q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q1 + L::PLANE));
+        }
+      };
+      if (more) {
         product(tb1, [&](int ks) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (r * KS / 16 == ks || (KS > 16 && r == ks)) exponential(r);
+            if (r * KS / 16 == ks) exponential(r);
         });
       } else {
 #pragma unroll
         for (int r = 0; r < 16; ++r) exponential(r);
       }
+      if (OUT) {
+#pragma unroll
+        for (int j = 0; j < AH; ++j) fetch2(j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       // second product, out^T += X^T P, with the conversion of the tile after next (behind the last tiles: of nothing, into a place
       // that nobody reads) and the next tile's exponents in its shadow
       if (OUT) {
-        typedef __attribute__((address_space(3))) s16x4* lp;
-        const Tile rt = ro.plus(tb * L::TILE);
-        constexpr int NS = 2 * DT, AH = BF16 ? (NS < 4 ? NS : 4) : 2;
-        XentFrag a[AH + 1], al[AH + 1];
-        const auto fetch = [&](int j) {
-          const int sk = j / DT, i = j % DT, chunk = i >> 1, rows = (chunk >> 1 < Tile::FULL ? 256 : 128);
-          const int x = 64 * (i & 1) | (rows == 256 ? (chunk & 1) << 7 : 0), from = 8192 * (chunk >> 1) + 16 * sk * rows;
-          const int r0 = rows == 256 ? rt.full : rt.half;
-          const char *q0 = lds.tile + (r0 ^ x) + from, *q1 = lds.tile + ((r0 + 8 * rows) ^ (x | 32)) + from;
-          a[j % (AH + 1)].q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q0);
-          a[j % (AH + 1)].q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q1);
-          if (!BF16) {
-            al[j % (AH + 1)].q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q0 + L::PLANE));
-            al[j % (AH + 1)].q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q1 + L::PLANE));
-          }
-        };
-#pragma unroll
-        for (int j = 0; j < AH; ++j) fetch(j);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
           const int sk = j / DT, i = j % DT;
-          if (j + AH < NS) fetch(j + AH);
-          o[i] = xent_mfma<BF16>(a[j % (AH + 1)], pf[0][sk], o[i]);
+          if (j + AH < NS) fetch2(j + AH);
+          o[i] = xent_mfma<BF16>(oa[j % (AH + 1)], pf[0][sk], o[i]);
           if (!BF16) {
-            o[i] = xent_mfma<BF16>(a[j % (AH + 1)], pf[PL - 1][sk], o[i]);
-            o[i] = xent_mfma<BF16>(al[j % (AH + 1)], pf[0][sk], o[i]);
+            o[i] = xent_mfma<BF16>(oa[j % (AH + 1)], pf[PL - 1][sk], o[i]);
+            o[i] = xent_mfma<BF16>(ol[j % (AH + 1)], pf[0][sk], o[i]);
           }
           if (!DMA) stage.step(j, lds.tile + tb2 * L::TILE, wr);
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (q * NS / 4 == j) exponents(q, ab1);
+          if (IS_DT && j == NS - 1) mark = __float_as_int(lds.rec[ab1].v[3][n]);
           XENT_MIX(BF16 ? 1 : 3);
         }
       }
@@ -733,12 +795,19 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
 #pragma unroll
       for (int q = 0; q < 4; ++q) exponents(q, ab1);
     }
-    factors(t + 2, ab2);
-    if (!DMA && t + 3 < tile1) load(t + 3, 0);
-    if (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (!DMA) {
+      factors(t + 2, ab2);
+      if (t + 3 < tile1) load(t + 3, 0, 0);
+    } else {
+      arrived();
+    }
     __syncthreads();
     tb = tb1;
     ab = ab1;
+  }
+  if (DMA) {                                     // LDS is used again below
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
   }
   if (!active) return;
   if (!IS_DT) l += __shfl_xor(l, 32);

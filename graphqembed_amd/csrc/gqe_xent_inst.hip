@@ -7,7 +7,7 @@
 
 template <int MODE, bool UNIT, bool DMA>
 static hipError_t launch(const XentPass& p, hipStream_t stream) {
-  typedef XentLds<GQE_XENT_BF16 != 0, GQE_XENT_DK, MODE> L;
+  typedef XentLds<GQE_XENT_BF16 != 0, GQE_XENT_DK, MODE, DMA> L;
   const void* f = (const void*)gqe_xent_kernel<GQE_XENT_BF16 != 0, GQE_XENT_DK, MODE, UNIT, DMA>;
   if (sizeof(L) > 65536) {
     const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(L));
@@ -36,3 +36,10 @@ hipError_t XENT_PREP_NAME(GQE_XENT_BF16, GQE_XENT_DK)(bool unit, const XentPrep&
   else gqe_xent_prep_kernel<GQE_XENT_BF16 != 0, GQE_XENT_DK, false><<<grid, dim3(256), 0, stream>>>(p);
   return hipGetLastError();
 }
+
+#if GQE_XENT_BF16 == 0 && GQE_XENT_DK == 64
+hipError_t gqe_xent_recs(const XentRecs& p, hipStream_t stream) {
+  gqe_xent_recs_kernel<0><<<dim3((unsigned)((p.n + 255) / 256)), dim3(256), 0, stream>>>(p);
+  return hipGetLastError();
+}
+#endif
