@@ -337,7 +337,7 @@ hipError_t xent_prep(bool bf16, int dk, bool unit, const XentPrep& p, hipStream_
 template <int MODE>
 void join_launch(bool bf16, const XentJoin& j, hipStream_t s) {
   const dim3 grid((unsigned)j.ny);
-  if (j.n_split > 8) {
+  if (j.n_split > (MODE == XENT_MODE_LSE ? 64 : 8)) {      // (losses alone: a wave reads 64 splits at once)
     if (bf16) gqe_xent_join_kernel<true, MODE, 8><<<grid, dim3(512), 0, s>>>(j);
     else gqe_xent_join_kernel<false, MODE, 8><<<grid, dim3(512), 0, s>>>(j);
   } else {

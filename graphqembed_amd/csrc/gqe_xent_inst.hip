@@ -1,4 +1,6 @@
 // One (type, padded dim) of the softmax cross entropy's kernels per translation unit: -DGQE_XENT_BF16=0|1 -DGQE_XENT_DK=64|128|192|256.
+#include <atomic>
+
 #include "gqe_xent.h"
 #include "gqe_ops_dev.h"
 
@@ -9,9 +11,15 @@ template <int MODE, bool UNIT, bool DMA>
 static hipError_t launch(const XentPass& p, hipStream_t stream) {
   typedef XentLds<GQE_XENT_BF16 != 0, GQE_XENT_DK, MODE, DMA> L;
   const void* f = (const void*)gqe_xent_kernel<GQE_XENT_BF16 != 0, GQE_XENT_DK, MODE, UNIT, DMA>;
-  if (sizeof(L) > 65536) {
-    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(L));
+  if (sizeof(L) > 65536) {            // once per device
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return e;
+    if (dev > 63 || !(done.load() >> dev & 1)) {
+      if ((e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(L))) != hipSuccess) return e;
+      if (dev <= 63) done.fetch_or((uint64_t)1 << dev);
+    }
   }
   gqe_xent_kernel<GQE_XENT_BF16 != 0, GQE_XENT_DK, MODE, UNIT, DMA><<<dim3((unsigned)(p.n_split * p.n_yblk)), dim3(256), sizeof(L), stream>>>(p);
   return hipGetLastError();

@@ -15,6 +15,8 @@ float32 (the norm: float64).  There is no CPU fallback: without libgqe.so or a H
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import struct
 from collections import OrderedDict
 
 import torch
@@ -49,16 +51,21 @@ class gqe_layer_norm_args(C.Structure):
                 ("workspace", _P), ("workspace_bytes", C.c_int64), ("stream", _P)]
 
 
+# The same as bytes (a call of 20 us cannot spend 5 of them on setting fields one by one); tests/test_ops_cpu.py holds the two together.
+_XENT = struct.Struct("@4i2qPqPqPPfiPPPPqiiPqPqP")
+_NORM = struct.Struct("@4iqPqPPfiPqPPPqPqPPPqP")
+_TENSOR = struct.Struct("@Pqii")
+
 # every symbol include/gqe_ops.h declares: name -> (restype, argtypes)
 OPS_SYMBOLS = OrderedDict([
     ("gqe_ops_last_error", (C.c_char_p, [])),
-    ("gqe_softmax_xent_workspace", (C.c_int64, [C.POINTER(gqe_xent_args)])),
-    ("gqe_softmax_xent", (C.c_int, [C.POINTER(gqe_xent_args)])),
-    ("gqe_clip_grads_workspace", (C.c_int64, [C.POINTER(gqe_tensor), C.c_int32])),
-    ("gqe_clip_grads", (C.c_int, [C.c_int32, C.POINTER(gqe_tensor), C.c_int32, C.c_float, _P, _P, C.c_int64, _P])),
-    ("gqe_layer_norm_workspace", (C.c_int64, [C.POINTER(gqe_layer_norm_args)])),
-    ("gqe_layer_norm_forward", (C.c_int, [C.POINTER(gqe_layer_norm_args)])),
-    ("gqe_layer_norm_backward", (C.c_int, [C.POINTER(gqe_layer_norm_args)])),
+    ("gqe_softmax_xent_workspace", (C.c_int64, [_P])),
+    ("gqe_softmax_xent", (C.c_int, [_P])),
+    ("gqe_clip_grads_workspace", (C.c_int64, [_P, C.c_int32])),
+    ("gqe_clip_grads", (C.c_int, [C.c_int32, _P, C.c_int32, C.c_float, _P, _P, C.c_int64, _P])),
+    ("gqe_layer_norm_workspace", (C.c_int64, [_P])),
+    ("gqe_layer_norm_forward", (C.c_int, [_P])),
+    ("gqe_layer_norm_backward", (C.c_int, [_P])),
 ])
 
 _lib = None
@@ -82,79 +89,90 @@ def _check(rc):
     return rc
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _on_gpu(what, *tensors):
-    """All tensors on one HIP device; its index."""
+    """Index of the HIP device that all tensors are on."""
+    index = None
     for t in tensors:
         if not isinstance(t, torch.Tensor):
             raise ValueError("%s: expected a tensor, got %s" % (what, type(t).__name__))
-        if not t.is_cuda:
+        i = t.get_device() if t.is_cuda else -1
+        if i < 0:
             raise GqeLibraryError("%s: the operators run on an MI355X only (got a tensor on %s; there is no CPU fallback)" % (what, t.device))
-        if t.device != tensors[0].device:
+        if index is None:
+            index = i
+        elif i != index:
             raise ValueError("%s: tensors on %s and %s" % (what, tensors[0].device, t.device))
-    return tensors[0].device
+    return index
 
 
 def _dtype(what, t):
-    if t.dtype not in _DTYPES:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         raise ValueError("%s: float32 or bfloat16, not %s" % (what, t.dtype))
-    return _DTYPES[t.dtype]
+    return code
 
 
 def _rows(t):
-    """[n, d] with unit stride along a row and rows that do not overlap (a view of a table keeps its row stride)."""
-    if t.shape[1] > 1 and t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
-
-
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+    """[n, d] with unit stride along a row and rows that do not overlap (a view of a table keeps its row stride), and that stride."""
+    n, d = t.shape
+    row, unit = t.stride()
+    if (d > 1 and unit != 1) or (n > 1 and row < d):
+        t, row = t.contiguous(), d
+    return t, max(row, d) if n <= 1 else row
 
 
 # -- softmax cross entropy over a table ----------------------------------------------------------------------------------------
 
-def _xent_args(what, q, table, target, scale, normalize):
-    dev = _on_gpu(what, q, table, target)
+@functools.lru_cache(maxsize=256)
+def _xent_space(phase, dtype, dim, n, rows, own_stat):
+    """Workspace bytes of a call: its sizes alone say."""
+    a = gqe_xent_args(phase=phase, dtype=dtype, dim=dim, n_queries=n, n_rows=rows, stat=1 if own_stat else None)
+    return _check(library().gqe_softmax_xent_workspace(C.byref(a)))
+
+
+def _xent(what, phase, q, table, target, scale, normalize, weight=None, loss=None, lse=None, stat=None, dq=None, dtable=None, accumulate=False):
+    """One call of gqe_softmax_xent on checked tensors; returns (q, table, target) as they were handed over."""
+    index = _on_gpu(what, q, table, target)
     if q.dim() != 2 or table.dim() != 2 or q.shape[1] != table.shape[1]:
         raise ValueError("%s: q [n, d] and table [rows, d], got %s and %s" % (what, tuple(q.shape), tuple(table.shape)))
     if q.dtype != table.dtype:
         raise ValueError("%s: q is %s, the table %s" % (what, q.dtype, table.dtype))
-    if target.dim() != 1 or target.shape[0] != q.shape[0] or target.dtype not in (torch.int32, torch.int64):
-        raise ValueError("%s: target is int32 or int64 [%d], got %s %s" % (what, q.shape[0], target.dtype, tuple(target.shape)))
-    if not 1 <= q.shape[1] <= MAX_DIM:
-        raise ValueError("%s: d = %d is not in 1 .. %d" % (what, q.shape[1], MAX_DIM))
-    if table.shape[0] < 1:
+    n, d = q.shape
+    rows = table.shape[0]
+    if target.dim() != 1 or target.shape[0] != n or target.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s: target is int32 or int64 [%d], got %s %s" % (what, n, target.dtype, tuple(target.shape)))
+    if not 1 <= d <= MAX_DIM:
+        raise ValueError("%s: d = %d is not in 1 .. %d" % (what, d, MAX_DIM))
+    if rows < 1:
         raise ValueError("%s: an empty table" % what)
     if target.dtype == torch.int64:       # rows beyond int32 (there are none) stay out of range
         target = target.clamp(-1, 0x7fffffff).to(torch.int32)
-    q, table, target = _rows(q), _rows(table), target.contiguous()
-    a = gqe_xent_args()
-    a.device, a.dtype, a.dim = dev.index, _dtype(what, q), q.shape[1]
-    a.n_queries, a.n_rows = q.shape[0], table.shape[0]
-    a.q, a.q_stride, a.table, a.table_stride = q.data_ptr(), _row_stride(q), table.data_ptr(), _row_stride(table)
-    a.target, a.scale, a.normalize = target.data_ptr(), float(scale), 1 if normalize else 0
-    return a, (q, table, target)
+    dtype = _dtype(what, q)
+    q, q_stride = _rows(q)
+    table, t_stride = _rows(table)
+    target = target.contiguous()
+    if weight is not None:
+        _on_gpu(what, q, weight)
+        if weight.dtype != torch.float32 or weight.dim() != 1 or weight.shape[0] != n:
+            raise ValueError("%s: weight is float32 [%d], got %s %s" % (what, n, weight.dtype, tuple(weight.shape)))
+        weight = weight.contiguous()
+    need = _xent_space(phase, dtype, d, n, rows, stat is not None)
+    space = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _check(library().gqe_softmax_xent(_XENT.pack(
+        index, phase, dtype, d, n, rows, q.data_ptr(), q_stride, table.data_ptr(), t_stride, target.data_ptr(),
+        0 if weight is None else weight.data_ptr(), scale, 1 if normalize else 0, 0 if loss is None else loss.data_ptr(),
+        0 if lse is None else lse.data_ptr(), 0 if stat is None else stat.data_ptr(), 0 if dq is None else dq.data_ptr(), d,
+        1 if dq is not None and dq.dtype == torch.float32 else 0, 1 if accumulate else 0, 0 if dtable is None else dtable.data_ptr(),
+        0 if dtable is None else max(dtable.stride(0), d) if rows <= 1 else dtable.stride(0), space.data_ptr(), need, _stream(index))))
+    return q, table, target
 
 
-def _xent_run(a, device):
-    lib = library()
-    need = _check(lib.gqe_softmax_xent_workspace(C.byref(a)))
-    space = torch.empty(need, dtype=torch.uint8, device=device)
-    a.workspace, a.workspace_bytes, a.stream = space.data_ptr(), need, _stream(device)
-    _check(lib.gqe_softmax_xent(C.byref(a)))
-
-
-def _weights(what, weight, q):
-    if weight is None:
-        return None
-    _on_gpu(what, q, weight)
-    if weight.dtype != torch.float32 or weight.shape != (q.shape[0],):
-        raise ValueError("%s: weight is float32 [%d], got %s %s" % (what, q.shape[0], weight.dtype, tuple(weight.shape)))
-    return weight.contiguous()
+def _floats(n, like):
+    return torch.empty(n, dtype=torch.float32, device=like.device)
 
 
 def softmax_xent_loss(q, table, target, scale=1.0, normalize=False):
@@ -162,11 +180,9 @@ def softmax_xent_loss(q, table, target, scale=1.0, normalize=False):
 
     ``normalize``: rows count as t / |t| (what the encoder does with the rows it reads; a zero row stays zero), so that unit queries
     score by cosine.  target < 0 ignores a query (loss 0; its lse is still given); target >= rows gives loss NaN."""
-    a, keep = _xent_args("softmax_xent_loss", q, table, target, scale, normalize)
-    loss = torch.empty(q.shape[0], dtype=torch.float32, device=q.device)
-    lse = torch.empty_like(loss)
-    a.phase, a.loss, a.lse = XENT_LOSS, loss.data_ptr(), lse.data_ptr()
-    _xent_run(a, q.device)
+    _on_gpu("softmax_xent_loss", q)
+    loss, lse = _floats(q.shape[0], q), _floats(q.shape[0], q)
+    _xent("softmax_xent_loss", XENT_LOSS, q, table, target, scale, normalize, loss=loss, lse=lse)
     return loss, lse
 
 
@@ -174,42 +190,34 @@ def softmax_xent_grads(q, table, target, weight=None, scale=1.0, normalize=False
     """(loss[n], lse[n], dq, dtable): ``softmax_xent_loss`` and the gradients of sum_b weight_b loss_b (None: all ones) in one call.
 
     dq and dtable have the type of q.  ``grad_table`` (float32, the table's shape): dtable is ADDED there instead, and returned."""
-    a, keep = _xent_args("softmax_xent_grads", q, table, target, scale, normalize)
-    n, d = q.shape
-    loss = torch.empty(n, dtype=torch.float32, device=q.device)
-    lse = torch.empty_like(loss)
-    dq = torch.empty((n, d), dtype=q.dtype, device=q.device)
-    w = _weights("softmax_xent_grads", weight, q)
-    if grad_table is None:
-        grad_table = torch.empty(tuple(table.shape), dtype=table.dtype, device=table.device)
+    what = "softmax_xent_grads"
+    _on_gpu(what, q, table)
+    loss, lse = _floats(q.shape[0], q), _floats(q.shape[0], q)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    accumulate = grad_table is not None
+    if not accumulate:
+        grad_table = torch.empty(table.shape, dtype=table.dtype, device=table.device)
     else:
-        _on_gpu("softmax_xent_grads", q, grad_table)
+        _on_gpu(what, q, grad_table)
+        d = table.shape[-1]
         if grad_table.dtype != torch.float32 or q.dtype != torch.float32 or grad_table.shape != table.shape or \
                 (d > 1 and grad_table.stride(1) != 1) or (table.shape[0] > 1 and grad_table.stride(0) < d):
-            raise ValueError("softmax_xent_grads: grad_table is float32 %s with unit stride along a row (and q float32)" % (tuple(table.shape),))
-        a.accumulate = 1
-    a.phase, a.loss, a.lse = XENT_LOSS | XENT_DQ | XENT_DTABLE, loss.data_ptr(), lse.data_ptr()
-    a.weight = None if w is None else w.data_ptr()
-    a.dq, a.dq_stride, a.dtable, a.dtable_stride = dq.data_ptr(), d, grad_table.data_ptr(), _row_stride(grad_table)
-    _xent_run(a, q.device)
+            raise ValueError("%s: grad_table is float32 %s with unit stride along a row (and q float32)" % (what, tuple(table.shape)))
+    _xent(what, XENT_LOSS | XENT_DQ | XENT_DTABLE, q, table, target, scale, normalize, weight=weight, loss=loss, lse=lse, dq=dq, dtable=grad_table,
+          accumulate=accumulate)
     return loss, lse, dq, grad_table
 
 
 class _SoftmaxXent(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, table, target, scale, normalize):
-        a, (qc, tc, tgt) = _xent_args("softmax_xent", q, table, target, scale, normalize)
-        n, d = q.shape
-        loss = torch.empty(n, dtype=torch.float32, device=q.device)
-        stat = torch.empty((n, 2), dtype=torch.float32, device=q.device)
-        dq = None
-        a.phase, a.loss, a.stat = XENT_LOSS, loss.data_ptr(), stat.data_ptr()
+        _on_gpu("softmax_xent", q, table)
+        loss, stat = _floats(q.shape[0], q), _floats((q.shape[0], 2), q)
+        dq, phase = None, XENT_LOSS
         if ctx.needs_input_grad[0]:
-            dq = torch.empty((n, d), dtype=torch.float32, device=q.device)      # of each query's own loss, scaled in backward
-            a.phase |= XENT_DQ
-            a.dq, a.dq_stride, a.dq_f32 = dq.data_ptr(), d, 1
-        _xent_run(a, q.device)
-        ctx.save_for_backward(qc, tc, tgt, stat, dq)
+            dq, phase = _floats(q.shape, q), XENT_LOSS | XENT_DQ      # of each query's own loss, scaled in backward
+        q, table, target = _xent("softmax_xent", phase, q, table, target, scale, normalize, loss=loss, stat=stat, dq=dq)
+        ctx.save_for_backward(q, table, target, stat, dq)
         ctx.scale, ctx.normalize = scale, normalize
         return loss
 
@@ -222,11 +230,8 @@ class _SoftmaxXent(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             gq = (dq * grad.unsqueeze(1)).to(q.dtype)
         if ctx.needs_input_grad[1]:
-            a, keep = _xent_args("softmax_xent", q, table, target, ctx.scale, ctx.normalize)
-            gt = torch.empty(tuple(table.shape), dtype=table.dtype, device=table.device)
-            a.phase, a.stat, a.weight = XENT_DTABLE, stat.data_ptr(), grad.data_ptr()
-            a.dtable, a.dtable_stride = gt.data_ptr(), _row_stride(gt)
-            _xent_run(a, q.device)
+            gt = torch.empty(table.shape, dtype=table.dtype, device=table.device)
+            _xent("softmax_xent", XENT_DTABLE, q, table, target, ctx.scale, ctx.normalize, weight=grad, stat=stat, dtable=gt)
         return gq, gt, None, None, None
 
 
@@ -249,17 +254,17 @@ def _clip(what, grads, max_norm):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if not grads:
         raise ValueError("%s: no tensors" % what)
-    dev = _on_gpu(what, *grads)
-    arr = (gqe_tensor * len(grads))()
-    for a, g in zip(arr, grads):
+    index = _on_gpu(what, *grads)
+    parts = []
+    for g in grads:
         if not g.is_contiguous():
             raise ValueError("%s: tensors are contiguous (got shape %s, strides %s)" % (what, tuple(g.shape), g.stride()))
-        a.data, a.numel, a.dtype = g.data_ptr(), g.numel(), _dtype(what, g)
-    lib = library()
-    need = _check(lib.gqe_clip_grads_workspace(arr, len(grads)))
-    space = torch.empty(need, dtype=torch.uint8, device=dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    _check(lib.gqe_clip_grads(dev.index, arr, len(grads), max_norm, norm.data_ptr(), space.data_ptr(), need, _stream(dev)))
+        parts.append(_TENSOR.pack(g.data_ptr(), g.numel(), _dtype(what, g), 0))
+    n, arr, lib = len(parts), b"".join(parts), library()
+    need = _check(lib.gqe_clip_grads_workspace(arr, n))
+    space = torch.empty(need, dtype=torch.uint8, device=grads[0].device)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _check(lib.gqe_clip_grads(index, arr, n, max_norm, norm.data_ptr(), space.data_ptr(), need, _stream(index)))
     return norm
 
 
@@ -279,64 +284,63 @@ def clip_grad_norm_(grads, max_norm):
 
 # -- layer normalisation -------------------------------------------------------------------------------------------------------
 
-def _ln_vector(what, name, v, x):
+def _ln_vector(what, name, v, index, d):
     if v is None:
-        return None
-    _on_gpu(what, x, v)
-    if v.dtype != torch.float32 or v.shape != (x.shape[-1],):
-        raise ValueError("%s: %s is float32 [%d], got %s %s" % (what, name, x.shape[-1], v.dtype, tuple(v.shape)))
-    return v.contiguous()
+        return 0
+    if _on_gpu(what, v) != index:
+        raise ValueError("%s: %s is on another device" % (what, name))
+    if v.dtype != torch.float32 or v.dim() != 1 or v.shape[0] != d or not (v.is_contiguous() or d == 1):
+        raise ValueError("%s: %s is float32 [%d], contiguous, got %s %s" % (what, name, d, v.dtype, tuple(v.shape)))
+    return v.data_ptr()
 
 
-def _ln_args(what, x):
-    if x.dim() != 2:
-        raise ValueError("%s: rows [n, d], got %s" % (what, tuple(x.shape)))
-    dev = _on_gpu(what, x)
-    a = gqe_layer_norm_args()
-    a.device, a.dtype, a.dim, a.n_rows = dev.index, _dtype(what, x), x.shape[1], x.shape[0]
-    x = _rows(x)
-    a.x, a.x_stride, a.stream = x.data_ptr(), _row_stride(x), _stream(dev)
-    return a, x
+@functools.lru_cache(maxsize=256)
+def _ln_space(dtype, dim, n):
+    """Workspace bytes of a backward call: its sizes alone say."""
+    a = gqe_layer_norm_args(dtype=dtype, dim=dim, n_rows=n)
+    return _check(library().gqe_layer_norm_workspace(C.byref(a)))
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     """(y, mean[n], rstd[n]) of the rows of x [n, d]; weight and bias float32 [d] or None; y has the type of x."""
-    a, x = _ln_args("layer_norm", x)
-    weight, bias = _ln_vector("layer_norm", "weight", weight, x), _ln_vector("layer_norm", "bias", bias, x)
+    what = "layer_norm"
+    index = _on_gpu(what, x)
+    if x.dim() != 2:
+        raise ValueError("%s: rows [n, d], got %s" % (what, tuple(x.shape)))
     n, d = x.shape
+    dtype = _dtype(what, x)
+    w, b = _ln_vector(what, "weight", weight, index, d), _ln_vector(what, "bias", bias, index, d)
+    x, stride = _rows(x)
     y = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    mean = torch.empty(n, dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
-    a.weight = None if weight is None else weight.data_ptr()
-    a.bias = None if bias is None else bias.data_ptr()
-    a.eps, a.y, a.y_stride, a.mean, a.rstd = float(eps), y.data_ptr(), d, mean.data_ptr(), rstd.data_ptr()
-    _check(library().gqe_layer_norm_forward(C.byref(a)))
+    mean, rstd = _floats(n, x), _floats(n, x)
+    _check(library().gqe_layer_norm_forward(_NORM.pack(index, dtype, d, 0, n, x.data_ptr(), stride, w, b, eps, 0, y.data_ptr(), d, mean.data_ptr(),
+                                                       rstd.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, _stream(index))))
     return y, mean, rstd
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None):
     """(dx, dweight, dbias) from the forward call's mean and rstd; dx has the type of x, dweight and dbias are float32."""
-    a, x = _ln_args("layer_norm_backward", x)
-    _on_gpu("layer_norm_backward", x, dy, mean, rstd)
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise ValueError("layer_norm_backward: dy is %s %s, x %s %s" % (dy.dtype, tuple(dy.shape), x.dtype, tuple(x.shape)))
-    for v in (mean, rstd):
-        if v.dtype != torch.float32 or v.shape != (x.shape[0],):
-            raise ValueError("layer_norm_backward: mean and rstd are float32 [%d]" % x.shape[0])
-    weight = _ln_vector("layer_norm_backward", "weight", weight, x)
-    dy, mean, rstd = _rows(dy), mean.contiguous(), rstd.contiguous()
+    what = "layer_norm_backward"
+    index = _on_gpu(what, x, dy, mean, rstd)
+    if x.dim() != 2 or dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("%s: rows [n, d] of one type, got dy %s %s, x %s %s" % (what, dy.dtype, tuple(dy.shape), x.dtype, tuple(x.shape)))
     n, d = x.shape
+    for v in (mean, rstd):
+        if v.dtype != torch.float32 or v.dim() != 1 or v.shape[0] != n:
+            raise ValueError("%s: mean and rstd are float32 [%d]" % (what, n))
+    dtype = _dtype(what, x)
+    w = _ln_vector(what, "weight", weight, index, d)
+    x, x_stride = _rows(x)
+    dy, dy_stride = _rows(dy)
+    mean, rstd = mean.contiguous(), rstd.contiguous()
     dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    cols = torch.empty((2, d), dtype=torch.float32, device=x.device)
-    lib = library()
-    need = _check(lib.gqe_layer_norm_workspace(C.byref(a)))
+    dweight, dbias = _floats(d, x), _floats(d, x)
+    need = _ln_space(dtype, d, n)
     space = torch.empty(need, dtype=torch.uint8, device=x.device)
-    a.weight = None if weight is None else weight.data_ptr()
-    a.mean, a.rstd, a.dy, a.dy_stride = mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), _row_stride(dy)
-    a.dx, a.dx_stride, a.dweight, a.dbias = dx.data_ptr(), d, cols[0].data_ptr(), cols[1].data_ptr()
-    a.workspace, a.workspace_bytes = space.data_ptr(), need
-    _check(lib.gqe_layer_norm_backward(C.byref(a)))
-    return dx, cols[0], cols[1]
+    _check(library().gqe_layer_norm_backward(_NORM.pack(index, dtype, d, 0, n, x.data_ptr(), x_stride, w, 0, 0.0, 0, 0, 0, mean.data_ptr(),
+                                                        rstd.data_ptr(), dy.data_ptr(), dy_stride, dx.data_ptr(), d, dweight.data_ptr(),
+                                                        dbias.data_ptr(), space.data_ptr(), need, _stream(index))))
+    return dx, dweight, dbias
 
 
 class _LayerNorm(torch.autograd.Function):

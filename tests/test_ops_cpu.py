@@ -61,14 +61,20 @@ def test_null_arguments(ops):
     assert lib.gqe_clip_grads(0, None, 3, 1.0, 1 << 20, 1 << 20, 1 << 30, None) == -1 and lib.gqe_clip_grads_workspace(None, 3) == -1
 
 
-def test_softmax_xent_workspace_grows_with_nothing_but_its_sizes(ops):
-    """No logits are kept: the workspace is bounded by a constant number of partial rows however large the table."""
+def test_softmax_xent_workspace(ops):
+    """No logits are kept: up to 128 queries the workspace is a constant number of partial rows however large the table; beyond, the
+    prepared operands come on top (as many bytes as float32 rows padded to 64 columns) with 24 bytes a row."""
     lib = ops.library()
     need = lambda **kw: lib.gqe_softmax_xent_workspace(C.byref(xent_args(ops, **kw)))
     assert need(dim=300) == -1
-    small, large = need(n_rows=10000, n_queries=512, dim=256), need(n_rows=100000000, n_queries=512, dim=256)
-    assert 0 < small and large < (256 + 8) * 128 * 4 * 300     # (slots + a few) x rows of a workgroup x (d + sums) x 4 bytes
-    assert need(n_rows=100000000, n_queries=512, dim=256, phase=1) < 1 << 20
+    parts = (256 + 8) * 128 * 4 * 300                           # (slots + a few) x rows of a workgroup x (d + sums) x 4 bytes
+    assert 0 < need(n_rows=10000, n_queries=128, dim=256) < parts
+    assert need(n_rows=100000000, n_queries=128, dim=256) < parts
+    for dim, padded in ((256, 256), (100, 128), (130, 192), (7, 64)):
+        big = need(n_rows=100000000, n_queries=512, dim=dim)
+        assert 100000000 * padded * 4 < big < 100000000 * (padded * 4 + 25) + 2 * parts
+        assert need(n_rows=100000000, n_queries=512, dim=dim, dtype=1) < 100000000 * (padded * 2 + 25) + 2 * parts
+    assert need(n_rows=100000000, n_queries=128, dim=256, phase=1) < 1 << 20
     assert need(n_queries=0) == 256
     assert need(n_rows=0x7fffff00, n_queries=0x7fffff00, dim=256, phase=2) > 0       # sizes stay in 64 bits
 
@@ -149,6 +155,11 @@ def test_the_binding_matches_the_header(ops):
                     names.append((part.strip().lstrip("* "), "p" if "*" in line else kind))
         types = {"int32_t": C.c_int32, "int64_t": C.c_int64, "float": C.c_float, "p": C.c_void_p}
         assert [(n, types[k]) for n, k in names] == getattr(ops, struct)._fields_
+    for struct, packed in (("gqe_xent_args", ops._XENT), ("gqe_tensor", ops._TENSOR), ("gqe_layer_norm_args", ops._NORM)):
+        kind = getattr(ops, struct)
+        values = [i + 1 for i in range(len(kind._fields_))]
+        a = kind.from_buffer_copy(packed.pack(*values))
+        assert C.sizeof(kind) == packed.size and [getattr(a, n) for n, _ in kind._fields_] == values
 
 
 def test_cpu_tensors_are_refused(ops):
