@@ -38,6 +38,7 @@ parser.add_argument("--model_dir", type=str, default="./")
 parser.add_argument("--decoder", type=str, default="bilinear")
 parser.add_argument("--inter_decoder", type=str, default="mean")
 parser.add_argument("--opt", type=str, default="adam")
+parser.add_argument("--max_grad_norm", type=float, default=None, help="scale each iteration's gradient to at most this norm")
 parser.add_argument("--seed", type=int, default=0)
 parser.add_argument("--flat", action="store_true", help="--data_dir was written by tools/convert_data.py --reddit")
 parser.add_argument("--make_synthetic", type=str, default=None, metavar="DIR")
@@ -85,7 +86,7 @@ enc = get_encoder(args.depth, graph, out_dims, feature_modules, args.cuda)
 dec = get_metapath_decoder(graph, out_dims, args.decoder)
 inter_dec = get_intersection_decoder(graph, out_dims, args.inter_decoder)
 enc_dec = QueryEncoderDecoder(graph, enc, dec, inter_dec)
-optimizer = FusedSGD(enc_dec, lr=args.lr) if args.opt == "sgd" else FusedAdam(enc_dec, lr=args.lr)
+optimizer = (FusedSGD if args.opt == "sgd" else FusedAdam)(enc_dec, lr=args.lr, max_grad_norm=args.max_grad_norm)
 name = "{data:s}-{depth:d}-{embed_dim:d}-{lr:f}-{decoder:s}-{inter_decoder:s}".format(
     data=args.data_dir.strip().rstrip("/").split("/")[-1], depth=args.depth, embed_dim=args.embed_dim, lr=args.lr, decoder=args.decoder,
     inter_decoder=args.inter_decoder)

@@ -492,3 +492,4 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
 
 #include "gqe_clip.h"
 #include "gqe_layer_norm.h"
+#include "gqe_chain.h"

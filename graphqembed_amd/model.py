@@ -19,9 +19,11 @@ import numpy as np
 import torch
 import torch.nn as nn
 
+from . import ops
 from .engine import ArenaLayout, Engine
+from .graph import CHAIN_TYPES
 from .tensorize import (FormulaPlan, pack_candidate_batches, pack_forward_batches, pack_margin_batches,
-                        reference_negative_nodes)
+                        reference_negative_nodes, rel_key, table_key)
 
 
 class _MarginLossFn(torch.autograd.Function):
@@ -51,16 +53,40 @@ class _MarginLossFn(torch.autograd.Function):
         return (None,) * 7
 
 
+class _SoftmaxLossFn(torch.autograd.Function):
+    """The same for the softmax loss over every entity: the backward call accumulates into the gradient arena."""
+
+    @staticmethod
+    def forward(ctx, anchor, model, formula, target, anchors, scale):
+        ctx.call = (model, formula, target, anchors, scale)
+        losses = model.softmax_losses(formula, target, anchors, scale)
+        n = int((target >= 1).sum())
+        return losses.sum() / max(n, 1)
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        model, formula, target, anchors, scale = ctx.call
+        model._prepare_grads(model._softmax_keys(formula))
+        model.softmax_step([(formula, target, anchors, float(grad_out.item()))], scale)
+        return (None,) * 6
+
+
 class QueryEncoderDecoder(nn.Module):
     """Encoder-decoder that scores conjunctive queries (edges, metapaths, intersections)."""
 
     def __init__(self, graph, enc, path_dec, inter_dec, device=None, max_queries=8192, max_batches=16, rank=0, world=1,
-                 lazy_adam=False):
+                 lazy_adam=False, query_norm=False):
+        """``query_norm``: the softmax losses over every entity (``softmax_step`` below) put a layer normalisation with a learned gain
+        and bias (parameters ``query_norm.weight`` / ``.bias``) between a chain's embedding and the scores: the embedding shrinks with
+        every relation it is multiplied by, the logits of a softmax over many entities have to stay of ordinary size.  The
+        reference's own scores and margin losses are not changed by it."""
         super(QueryEncoderDecoder, self).__init__()
         self.enc = enc
         self.path_dec = path_dec
         self.inter_dec = inter_dec
         self.graph = graph
+        if query_norm:
+            self.query_norm = nn.LayerNorm(next(enc.parameters()).shape[-1])      # owns the parameters; ops.layer_norm computes
         layout = ArenaLayout()
         dims = set()
         for name, p in self.named_parameters():
@@ -184,6 +210,10 @@ class QueryEncoderDecoder(nn.Module):
         point settles it; ``state_dict()`` / ``sync()`` do so before values are read through the ``nn.Parameter`` views)."""
         if not isinstance(optimizer, FusedAdam) or optimizer.model is not self:
             raise Exception("train_step needs this model's FusedAdam")
+        if optimizer.max_grad_norm is not None:       # the norm is known behind the whole backward pass only
+            losses, _, _ = self.margin_step(items, idx_device=idx_device)
+            optimizer.step()
+            return losses
         packed = [(self.plan(f), t, ng, a, w, m) for (f, t, ng, a, w, m) in items]
         descs, idx, _ = pack_margin_batches(packed)
         keys = set(self._touched)          # (gradients an earlier margin_loss / margin_step left behind are stepped too)
@@ -258,6 +288,99 @@ class QueryEncoderDecoder(nn.Module):
             off += len(r)
         return self.engine.rank_candidates(scores, np.concatenate(ptr).astype(np.int32))
 
+    # -- every entity of the target mode as the candidates of a chain query (ops.py) --------------------------------------
+    # score(b, v) = scale * f(q_b) . t_v / |t_v| over the table rows v = 1 .. (row 0 is the dummy), q_b the anchor's unit row times the
+    # chain's relation vectors (decoders.py:228-233), f the layer normalisation of ``query_norm`` or nothing.
+    def _softmax_check(self, formula):
+        what = "the softmax loss over every entity"
+        if formula.query_type not in CHAIN_TYPES or self.path_dec.kind != "bilinear-diag":
+            raise Exception("%s takes chain queries of the bilinear-diag decoder, not %s of %s" % (what, formula.query_type, self.path_dec.kind))
+        bags = getattr(self.enc, "bag_csr", {})
+        for m in (formula.target_mode,) + tuple(formula.anchor_modes):
+            if m in bags:
+                raise Exception("%s: mode %r is an EmbeddingBag, its entities are no table rows" % (what, m))
+        if self.engine.world > 1 or self.engine.sharded:
+            raise Exception("%s runs on one GPU (whole tables, no gradient exchange)" % what)
+
+    def _softmax_keys(self, formula):
+        self._softmax_check(formula)
+        keys = {table_key(formula.target_mode), table_key(formula.anchor_modes[0])}
+        keys.update(rel_key(r) for r in formula.rels)
+        if hasattr(self, "query_norm"):
+            keys.update(("query_norm.weight", "query_norm.bias"))
+        return keys
+
+    def _softmax_feed(self, items):
+        """One upload for all batches: (anchor rows, candidates = target rows - 1, weight_b = loss weight / queries) of each."""
+        parts, counts = [], []
+        for formula, target, anchors, weight in items:
+            target = np.ascontiguousarray(target, dtype=np.int32)
+            anchors = np.ascontiguousarray(np.asarray(anchors, dtype=np.int32).reshape(-1))
+            rows = [self.layout.entries[table_key(m)][1][0] for m in (formula.target_mode, formula.anchor_modes[0])]
+            if len(target) != len(anchors):
+                raise Exception("%d target and %d anchor rows" % (len(target), len(anchors)))
+            for r, hi in ((target, rows[0]), (anchors, rows[1])):
+                if len(r) and (r.min() < 0 or r.max() >= hi):
+                    raise Exception("a row outside 0 .. %d" % (hi - 1))
+            counts.append((len(target), max(int((target >= 1).sum()), 1)))
+            parts.extend((anchors, target - 1, np.full(len(target), weight / counts[-1][1], dtype=np.float32).view(np.int32)))
+        flat = torch.from_numpy(np.concatenate(parts)).to(self.engine.device)
+        out, off = [], 0
+        for n, real in counts:
+            out.append((flat[off:off + n], flat[off + n:off + 2 * n], flat[off + 2 * n:off + 3 * n].view(torch.float32), real))
+            off += 3 * n
+        return out
+
+    def _softmax_query(self, formula, rows):
+        """(f(q), what backward needs)"""
+        view = lambda k: self.layout.view(self.engine._params, k)
+        table, rels = view(table_key(formula.anchor_modes[0])), [view(rel_key(r)) for r in formula.rels]
+        q = ops.chain_rows(table, rows, rels)
+        if not hasattr(self, "query_norm"):
+            return q, (q, None, None)
+        y, mean, rstd = ops.layer_norm_forward(q, view("query_norm.weight"), view("query_norm.bias"), self.query_norm.eps)
+        return y, (q, mean, rstd)
+
+    def softmax_losses(self, formula, target_rows, anchor_rows, scale=1.0):
+        """Each query's -log softmax over every entity of the target mode (a device tensor [n], no gradient; 0 for the dummy row 0)."""
+        self._softmax_check(formula)
+        self.engine.sync()
+        rows, target, _, _ = self._softmax_feed([(formula, target_rows, anchor_rows, 1.0)])[0]
+        q, _ = self._softmax_query(formula, rows)
+        return ops.softmax_xent_loss(q, self.layout.view(self.engine._params, table_key(formula.target_mode))[1:], target, scale, True)[0]
+
+    def softmax_loss(self, formula, queries, scale=1.0):
+        """``margin_loss`` against every entity at once instead of one sampled negative: the mean of -log softmax at the queries'
+        targets, differentiable like ``margin_loss`` (the gradients appear as ``param.grad``)."""
+        target, anchors = self._rows(formula, queries, [q.target_node for q in queries])
+        return _SoftmaxLossFn.apply(self._autograd_anchor, self, formula, target, anchors, float(scale))
+
+    def softmax_step(self, items, scale=1.0):
+        """``margin_step`` against every entity at once: items [(formula, target_rows[n], anchor_rows[1, n], loss_weight)] of chain
+        queries; accumulates d(sum_i w_i loss_i) into the gradient arena, loss_i the mean over the batch's queries, and returns
+        losses[len(items) + 1] (their weighted sum last).  ``optimizer.step()`` follows, and any margin_step may join it.  The whole
+        target table has a gradient: the optimiser's pass covers all of its rows."""
+        keys = [self._softmax_keys(item[0]) for item in items]
+        eng = self.engine
+        feed = self._softmax_feed(items)
+        eng.sync()
+        eng.materialize()       # lists of an earlier margin_step join the dense gradients; the next optimiser pass reads those
+        grad = lambda k: self.layout.view(eng.grads, k)
+        param = lambda k: self.layout.view(eng._params, k)
+        losses = torch.zeros(len(items) + 1, dtype=torch.float32, device=eng.device)
+        for i, ((formula, _, _, weight), (rows, target, w, real)) in enumerate(zip(items, feed)):
+            q, (raw, mean, rstd) = self._softmax_query(formula, rows)
+            t = table_key(formula.target_mode)
+            loss, _, dq, _ = ops.softmax_xent_grads(q, param(t)[1:], target, weight=w, scale=scale, normalize=True, grad_table=grad(t)[1:])
+            if mean is not None:
+                dq, _, _ = ops.layer_norm_backward(dq, raw, mean, rstd, param("query_norm.weight"), grad("query_norm.weight"), grad("query_norm.bias"))
+            a = table_key(formula.anchor_modes[0])
+            ops.chain_rows_backward(dq, param(a), rows, [param(rel_key(r)) for r in formula.rels], grad(a), [grad(rel_key(r)) for r in formula.rels])
+            torch.mul(loss.sum(), 1.0 / real, out=losses[i])
+            losses[-1].add_(losses[i], alpha=float(weight))
+            self._mark_touched(keys[i])
+        return losses
+
     def score_batches(self, items):
         """items: [(formula, target_rows, anchor_rows)] -> one scores tensor (concatenated)."""
         packed = [(self.plan(f), t, a) for (f, t, a) in items]
@@ -271,9 +394,25 @@ class _FusedOptimizer(object):
     received a gradient this iteration (torch semantics: others are skipped and keep their
     own step count — SURVEY.md Appendix B)."""
 
-    def __init__(self, model, lr):
+    def __init__(self, model, lr, max_grad_norm=None):
+        """``max_grad_norm``: ``step`` first scales the gradients of the touched tensors to at most this norm over all of them
+        (ops.clip_grad_norm_); ``grad_norm`` is then the norm before (a 0-dim device tensor)."""
+        if max_grad_norm is not None:
+            max_grad_norm = float(max_grad_norm)
+            if not max_grad_norm >= 0.0:
+                raise ValueError("max_grad_norm %r" % (max_grad_norm,))
+            if model.engine.world > 1 or model.engine.sharded:
+                raise Exception("max_grad_norm needs the whole gradient on one GPU: not with a gradient exchange or row-sharded tables")
         self.model = model
         self.lr = lr
+        self.max_grad_norm, self.grad_norm = max_grad_norm, None
+
+    def _clip(self):
+        m, eng = self.model, self.model.engine
+        if self.max_grad_norm is None or not m._touched:
+            return
+        eng.materialize()         # the rows' gradient lists become dense gradients: what the norm is of
+        self.grad_norm = ops.clip_grad_norm_([m.layout.view(eng.grads, k) for k in m.layout.entries if k in m._touched], self.max_grad_norm)
 
     def zero_grad(self, set_to_none=True):
         m = self.model
@@ -295,12 +434,13 @@ class _FusedOptimizer(object):
 class FusedAdam(_FusedOptimizer):
     """torch.optim.Adam(lr, betas=(0.9,0.999), eps=1e-8) (netquery/bio/train.py:62)."""
 
-    def __init__(self, model, lr=0.01, betas=(0.9, 0.999), eps=1e-8):
-        _FusedOptimizer.__init__(self, model, lr)
+    def __init__(self, model, lr=0.01, betas=(0.9, 0.999), eps=1e-8, max_grad_norm=None):
+        _FusedOptimizer.__init__(self, model, lr, max_grad_norm)
         self.betas, self.eps = betas, eps
 
     def step(self):
         m = self.model
+        self._clip()
         if m._touched:
             m.engine.adam_step(m._touched, self.lr, self.betas, self.eps)
         self._done()
@@ -331,6 +471,7 @@ class FusedSGD(_FusedOptimizer):
 
     def step(self):
         m = self.model
+        self._clip()
         if m._touched:
             m.engine.sgd_step(m._touched, self.lr)
         self._done()

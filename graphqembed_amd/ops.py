@@ -6,6 +6,7 @@ entity needs next to it:
     softmax_xent, softmax_xent_loss, softmax_xent_grads   cross entropy of a softmax over all rows of a table, logits never kept
     grad_norm, clip_grad_norm_                            global gradient norm over many tensors, clipping in place
     layer_norm, layer_norm_forward, layer_norm_backward   layer normalisation of query rows
+    chain_rows, chain_rows_backward                       query embeddings of a bilinear-diag relation chain
 
 ``softmax_xent`` and ``layer_norm`` are differentiable by torch's autograd; the others are the calls a fused training step makes.
 All work is enqueued on ``torch.cuda.current_stream()`` of the tensors' device (which need not be the current device); nothing
@@ -51,6 +52,13 @@ class gqe_layer_norm_args(C.Structure):
                 ("workspace", _P), ("workspace_bytes", C.c_int64), ("stream", _P)]
 
 
+class gqe_chain_args(C.Structure):
+    _fields_ = [("device", C.c_int32), ("dim", C.c_int32), ("n", C.c_int64), ("rows", _P), ("table", _P), ("table_stride", C.c_int64),
+                ("n_rows", C.c_int64), ("n_rels", C.c_int32), ("reserved", C.c_int32), ("rel", _P * 3), ("q", _P), ("q_stride", C.c_int64),
+                ("dq", _P), ("dq_stride", C.c_int64), ("dtable", _P), ("dtable_stride", C.c_int64), ("drel", _P * 3),
+                ("workspace", _P), ("workspace_bytes", C.c_int64), ("stream", _P)]
+
+
 # The same as bytes (a call of 20 us cannot spend 5 of them on setting fields one by one); tests/test_ops_cpu.py holds the two together.
 _XENT = struct.Struct("@4i2qPqPqPPfiPPPPqiiPqPqP")
 _NORM = struct.Struct("@4iqPqPPfiPqPPPqPqPPPqP")
@@ -66,6 +74,8 @@ OPS_SYMBOLS = OrderedDict([
     ("gqe_layer_norm_workspace", (C.c_int64, [_P])),
     ("gqe_layer_norm_forward", (C.c_int, [_P])),
     ("gqe_layer_norm_backward", (C.c_int, [_P])),
+    ("gqe_chain_rows_forward", (C.c_int, [_P])),
+    ("gqe_chain_rows_backward", (C.c_int, [_P])),
 ])
 
 _lib = None
@@ -318,8 +328,10 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     return y, mean, rstd
 
 
-def layer_norm_backward(dy, x, mean, rstd, weight=None):
-    """(dx, dweight, dbias) from the forward call's mean and rstd; dx has the type of x, dweight and dbias are float32."""
+def layer_norm_backward(dy, x, mean, rstd, weight=None, grad_weight=None, grad_bias=None):
+    """(dx, dweight, dbias) from the forward call's mean and rstd; dx has the type of x, dweight and dbias are float32.
+
+    ``grad_weight`` and ``grad_bias`` (float32 [d], both or neither): the two are ADDED there instead, and returned."""
     what = "layer_norm_backward"
     index = _on_gpu(what, x, dy, mean, rstd)
     if x.dim() != 2 or dy.shape != x.shape or dy.dtype != x.dtype:
@@ -334,10 +346,16 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None):
     dy, dy_stride = _rows(dy)
     mean, rstd = mean.contiguous(), rstd.contiguous()
     dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    dweight, dbias = _floats(d, x), _floats(d, x)
+    accumulate = grad_weight is not None
+    if accumulate != (grad_bias is not None):
+        raise ValueError("%s: grad_weight and grad_bias come together" % what)
+    if accumulate:
+        _ln_vector(what, "grad_weight", grad_weight, index, d)
+        _ln_vector(what, "grad_bias", grad_bias, index, d)
+    dweight, dbias = (grad_weight, grad_bias) if accumulate else (_floats(d, x), _floats(d, x))
     need = _ln_space(dtype, d, n)
     space = torch.empty(need, dtype=torch.uint8, device=x.device)
-    _check(library().gqe_layer_norm_backward(_NORM.pack(index, dtype, d, 0, n, x.data_ptr(), x_stride, w, 0, 0.0, 0, 0, 0, mean.data_ptr(),
+    _check(library().gqe_layer_norm_backward(_NORM.pack(index, dtype, d, 1 if accumulate else 0, n, x.data_ptr(), x_stride, w, 0, 0.0, 0, 0, 0, mean.data_ptr(),
                                                         rstd.data_ptr(), dy.data_ptr(), dy_stride, dx.data_ptr(), d, dweight.data_ptr(),
                                                         dbias.data_ptr(), space.data_ptr(), need, _stream(index))))
     return dx, dweight, dbias
@@ -364,3 +382,54 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if x.dim() < 1:
         raise ValueError("layer_norm: a 0-dim tensor")
     return _LayerNorm.apply(x.reshape(-1, x.shape[-1]), weight, bias, float(eps)).view(x.shape)
+
+
+# -- query side of a relation chain ----------------------------------------------------------------------------------------------
+
+def _chain_args(what, table, rows, rels):
+    index = _on_gpu(what, table, rows, *rels)
+    d = table.shape[-1]
+    if table.dim() != 2 or table.dtype != torch.float32 or not 1 <= d <= MAX_DIM or (d > 1 and table.stride(1) != 1) or table.shape[0] < 1 or \
+            (table.shape[0] > 1 and table.stride(0) < d):
+        raise ValueError("%s: the table is float32 [rows, d <= %d] with unit stride along a row" % (what, MAX_DIM))
+    if rows.dim() != 1 or rows.dtype != torch.int32 or not rows.is_contiguous():
+        raise ValueError("%s: rows is int32 [n], contiguous" % what)
+    if len(rels) > 3:
+        raise ValueError("%s: %d relations" % (what, len(rels)))
+    a = gqe_chain_args()
+    a.device, a.dim, a.n, a.rows = index, d, rows.shape[0], rows.data_ptr()
+    a.table, a.table_stride, a.n_rows, a.n_rels, a.stream = table.data_ptr(), max(table.stride(0), d), table.shape[0], len(rels), _stream(index)
+    for j, r in enumerate(rels):
+        if r.dtype != torch.float32 or r.dim() != 1 or r.shape[0] != d or not r.is_contiguous():
+            raise ValueError("%s: relations are float32 [%d], contiguous" % (what, d))
+        a.rel[j] = r.data_ptr()
+    return a
+
+
+def chain_rows(table, rows, rels):
+    """q [n, d]: the anchors' table rows over their lengths, times the relation vectors (at most 3) element by element."""
+    a = _chain_args("chain_rows", table, rows, rels)
+    q = torch.empty((a.n, a.dim), dtype=torch.float32, device=table.device)
+    a.q, a.q_stride = q.data_ptr(), a.dim
+    _check(library().gqe_chain_rows_forward(C.byref(a)))
+    return q
+
+
+def chain_rows_backward(dq, table, rows, rels, grad_table, grad_rels):
+    """ADD the gradients of ``chain_rows`` into grad_table (the table's shape) and grad_rels (one for each relation)."""
+    what = "chain_rows_backward"
+    a = _chain_args(what, table, rows, rels)
+    _on_gpu(what, table, dq, grad_table, *grad_rels)
+    if dq.dtype != torch.float32 or dq.dim() != 2 or tuple(dq.shape) != (a.n, a.dim) or grad_table.dtype != torch.float32 or grad_table.shape != table.shape or \
+            (a.dim > 1 and grad_table.stride(1) != 1) or (a.n_rows > 1 and grad_table.stride(0) < a.dim) or len(grad_rels) != len(rels):
+        raise ValueError("%s: dq is float32 [%d, %d], the gradients have their tensors' shapes" % (what, a.n, a.dim))
+    for j, r in enumerate(grad_rels):
+        if r.dtype != torch.float32 or r.dim() != 1 or r.shape[0] != a.dim or not r.is_contiguous():
+            raise ValueError("%s: gradients of relations are float32 [%d], contiguous" % (what, a.dim))
+        a.drel[j] = r.data_ptr()
+    dq, stride = _rows(dq)
+    need = 8 * a.n * a.dim
+    space = torch.empty(max(need, 4), dtype=torch.uint8, device=table.device)
+    a.dq, a.dq_stride, a.dtable, a.dtable_stride = dq.data_ptr(), stride, grad_table.data_ptr(), max(grad_table.stride(0), a.dim)
+    a.workspace, a.workspace_bytes = space.data_ptr(), need
+    _check(library().gqe_chain_rows_backward(C.byref(a)))

@@ -124,7 +124,8 @@ class FusedExecutor(object):
         library call (model.train_step: gqe_train_step), and the loop's ``optimizer.step()`` finds nothing left to do."""
         self.model = model
         self.optimizer = optimizer if isinstance(optimizer, FusedAdam) else None
-        self.native_optimizer = optimizer if isinstance(optimizer, (FusedAdam, FusedSGD)) else None    # (what the native loop can step with)
+        # (what the native loop can step with; a norm over the whole gradient it does not take)
+        self.native_optimizer = optimizer if isinstance(optimizer, (FusedAdam, FusedSGD)) and optimizer.max_grad_norm is None else None
         self.items = []
         self._full = {}           # mode -> rows of graph.full_lists[mode] (1-chain negatives)
 

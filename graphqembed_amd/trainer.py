@@ -43,7 +43,7 @@ class PoolView(object):
 
 class TensorizedTrainer(object):
     def __init__(self, model_or_engine, optimizer, pools_by_type, all_rows_by_mode, batch_size=512, inter_weight=0.005,
-                 path_weight=0.01, seed=0, plan_of=None, dist=None, rank=0, world=1, engine=None):
+                 path_weight=0.01, seed=0, plan_of=None, dist=None, rank=0, world=1, engine=None, loss="margin", softmax_scale=1.0):
         """pools_by_type: {query_type: [pool, ...]} (one pool per formula); all_rows_by_mode: {mode: int32 rows}
         to draw 1-chain negatives from.  ``model_or_engine``: a QueryEncoderDecoder (``margin_step``) — or any
         object with the same ``margin_step(items)`` method.
@@ -73,6 +73,17 @@ class TensorizedTrainer(object):
         self.engine = engine if engine is not None else getattr(model_or_engine, "engine", None)
         if self.world > 1 and (self.dist is None or self.engine is None):
             raise Exception("data-parallel training needs dist= and an Engine (model.engine or engine=)")
+        if loss not in ("margin", "softmax"):
+            raise Exception("loss is \"margin\" or \"softmax\", not %r" % (loss,))
+        self.loss, self.softmax_scale = loss, float(softmax_scale)
+        if loss == "softmax":
+            if self.world > 1 or not hasattr(model_or_engine, "softmax_step"):
+                raise Exception("loss=\"softmax\" trains a QueryEncoderDecoder on one GPU")
+            for t in self.types:
+                for p in self.pools[t]:
+                    model_or_engine._softmax_check(p.formula)
+        if getattr(optimizer, "max_grad_norm", None) is not None and self.world > 1:
+            raise Exception("max_grad_norm needs the whole gradient on one GPU")
         self._slab = 0
         self.plan_of = plan_of
         self.sharded = self.engine is not None and getattr(self.engine, "sharded", False)
@@ -102,6 +113,8 @@ class TensorizedTrainer(object):
         if self.world > 1:   # mean over the global batch = sum_r (n_r / n_all) * mean_r
             n_all = sum(e - s for s, e in (parallel.rank_slice(n, B, it, r, self.world) for r in range(self.world)))
             weight = weight * (end - start) / float(n_all)
+        if self.loss == "softmax":
+            return (p.formula, p.target[start:end], p.anchors[:, start:end], weight)
         all_rows = self.all_rows[p.formula.target_mode] if qtype == "1-chain" else None
         neg = p.negatives(start, end, hard, self.neg_rng, all_rows)
         return (p.formula, p.target[start:end], neg, p.anchors[:, start:end], weight, 1.0)
@@ -129,6 +142,12 @@ class TensorizedTrainer(object):
             if slab != self._slab:
                 self.engine.exchange_reserve(slab)
                 self._slab = slab
+        if self.loss == "softmax":
+            losses = self.model.softmax_step(items, self.softmax_scale)
+            self.opt.step()
+            self.iterations += 1
+            self.queries_seen += sum(len(x[1]) for x in items)
+            return losses
         if self._one_call:     # one GPU, the model's own FusedAdam: the iteration as ONE library call (gqe_train_step)
             losses = self.model.train_step(items, self.opt)
             self.iterations += 1

@@ -116,6 +116,35 @@ int64_t gqe_layer_norm_workspace(const gqe_layer_norm_args* args);
 int gqe_layer_norm_forward(const gqe_layer_norm_args* args);
 int gqe_layer_norm_backward(const gqe_layer_norm_args* args);
 
+/* ---- the query side of a relation chain -------------------------------------------------------------------------------------
+ * q_b = (w / |w|) r_1 .. r_k element by element, w = table row rows[b]: the bilinear-diag score of a chain (decoders.py:228-233) is q_b . t
+ * for every target t, so this is what gqe_softmax_xent scores against a whole table.  A row outside 0 .. n_rows - 1 gives NaN and no
+ * gradient.  Backward: ADDS into dtable and drel[j] (which may name one relation more than once).  float32; n <= 65536; workspace of the
+ * backward call: 8 n dim bytes. */
+typedef struct {
+  int32_t device;
+  int32_t dim;
+  int64_t n;
+  const int32_t* rows;      /* [n] */
+  const float* table;
+  int64_t table_stride, n_rows;
+  int32_t n_rels;           /* 0 .. 3 */
+  int32_t reserved;
+  const float* rel[3];
+  float* q;                 /* forward */
+  int64_t q_stride;
+  const float* dq;          /* backward */
+  int64_t dq_stride;
+  float* dtable;
+  int64_t dtable_stride;
+  float* drel[3];
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} gqe_chain_args;
+int gqe_chain_rows_forward(const gqe_chain_args* args);
+int gqe_chain_rows_backward(const gqe_chain_args* args);
+
 #ifdef __cplusplus
 }
 #endif

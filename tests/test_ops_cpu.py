@@ -139,12 +139,60 @@ def test_clip_grads_refuses_small_workspaces(ops):
     assert lib.gqe_clip_grads(0, arr, 1, 1.0, None, 1 << 20, need, None) == -1
 
 
+CHAIN_REFUSED = [("dim", dict(dim=0)), ("dim", dict(dim=257)), ("queries", dict(n=-1)), ("queries", dict(n=65537)), ("table", dict(n_rows=0)),
+                 ("relations", dict(n_rels=4)), ("relations", dict(n_rels=-1)), ("relation 0", dict(n_rels=1, rel=(C.c_void_p * 3)())),
+                 ("NULL", dict(table=None)), ("NULL", dict(rows=None)), ("stride", dict(table_stride=63))]
+
+
+@pytest.mark.parametrize("word,change", CHAIN_REFUSED + [("NULL", dict(q=None)), ("stride", dict(q_stride=3)), ("NULL", dict(dq=None)),
+                                                         ("relation 1", dict(drel=(C.c_void_p * 3)(1 << 20, None, None))), ("NULL", dict(dtable=None)),
+                                                         ("stride", dict(dtable_stride=1)), ("workspace", dict(workspace_bytes=8 * 10 * 64 - 1)),
+                                                         ("workspace", dict(workspace=None))])
+def test_chain_rows_refusals(ops, word, change):
+    lib = ops.library()
+    a = ops.gqe_chain_args(dim=64, n=10, n_rows=100, n_rels=2, workspace_bytes=1 << 20)
+    a.rows = a.table = a.q = a.dq = a.dtable = a.workspace = 1 << 20
+    a.table_stride = a.q_stride = a.dq_stride = a.dtable_stride = 64
+    a.rel = a.drel = (C.c_void_p * 3)(1 << 20, 1 << 20, None)
+    for k, v in change.items():
+        setattr(a, k, v)
+    both = [(lib.gqe_chain_rows_forward, ("q", "q_stride")), (lib.gqe_chain_rows_backward, ("dq", "drel", "dtable", "dtable_stride", "workspace", "workspace_bytes"))]
+    only = [fn for fn, fields in both if set(fields) & set(change)]
+    for fn in only or [fn for fn, _ in both]:
+        assert fn(C.byref(a)) == (-5 if word == "workspace" else -1)
+        assert word in lib.gqe_ops_last_error().decode()
+    assert lib.gqe_chain_rows_forward(None) == -1 and lib.gqe_chain_rows_backward(None) == -1
+
+
+def test_the_optimisers_and_the_trainer_refuse(ops):
+    """max_grad_norm and the softmax loss need whole gradients and whole tables: refused before anything runs."""
+    from graphqembed_amd.model import FusedAdam, FusedSGD
+    from graphqembed_amd.trainer import TensorizedTrainer
+
+    class Engine(object):
+        world, sharded = 2, False
+
+    class Model(object):
+        engine = Engine()
+    for kind in (FusedAdam, FusedSGD):
+        assert kind(Model(), lr=0.1).max_grad_norm is None
+        with pytest.raises(Exception, match="one GPU"):
+            kind(Model(), lr=0.1, max_grad_norm=1.0)
+        for bad in (-1.0, float("nan")):
+            with pytest.raises(ValueError):
+                kind(Model(), lr=0.1, max_grad_norm=bad)
+    with pytest.raises(Exception, match="loss"):
+        TensorizedTrainer(Model(), FusedSGD(Model(), 0.1), {}, {}, loss="softmax")
+    with pytest.raises(Exception, match="loss"):
+        TensorizedTrainer(Model(), FusedSGD(Model(), 0.1), {}, {}, loss="nce")
+
+
 def test_the_binding_matches_the_header(ops):
     text = open(os.path.join(ROOT, "include", "gqe_ops.h")).read()
     code = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     declared = set(re.findall(r"\b(gqe_\w+)\(", code))
     assert declared == set(ops.OPS_SYMBOLS)
-    for struct in ("gqe_xent_args", "gqe_tensor", "gqe_layer_norm_args"):
+    for struct in ("gqe_xent_args", "gqe_tensor", "gqe_layer_norm_args", "gqe_chain_args"):
         body = re.search(r"typedef struct \{([^{}]*)\} %s;" % struct, code).group(1)
         names = []
         for line in body.split(";"):
@@ -152,8 +200,9 @@ def test_the_binding_matches_the_header(ops):
             if line:
                 kind = re.match(r"(?:const )?(int32_t|int64_t|float|void)\b", line).group(1)
                 for part in line[line.index(kind) + len(kind):].split(","):
-                    names.append((part.strip().lstrip("* "), "p" if "*" in line else kind))
-        types = {"int32_t": C.c_int32, "int64_t": C.c_int64, "float": C.c_float, "p": C.c_void_p}
+                    name, count = re.match(r"(\w+)(?:\[(\d+)\])?$", part.strip().lstrip("* ")).groups()
+                    names.append((name, ("p" if "*" in line else kind) + (count or "")))
+        types = {"int32_t": C.c_int32, "int64_t": C.c_int64, "float": C.c_float, "p": C.c_void_p, "p3": C.c_void_p * 3}
         assert [(n, types[k]) for n, k in names] == getattr(ops, struct)._fields_
     for struct, packed in (("gqe_xent_args", ops._XENT), ("gqe_tensor", ops._TENSOR), ("gqe_layer_norm_args", ops._NORM)):
         kind = getattr(ops, struct)
@@ -167,7 +216,8 @@ def test_cpu_tensors_are_refused(ops):
     from graphqembed_amd.engine import GqeLibraryError
     q, t, tgt = torch.randn(3, 8), torch.randn(5, 8), torch.zeros(3, dtype=torch.int32)
     for call in (lambda: ops.softmax_xent_loss(q, t, tgt), lambda: ops.softmax_xent_grads(q, t, tgt), lambda: ops.softmax_xent(q, t, tgt),
-                 lambda: ops.clip_grad_norm_([q], 1.0), lambda: ops.grad_norm([q]), lambda: ops.layer_norm(q), lambda: ops.layer_norm_forward(q)):
+                 lambda: ops.clip_grad_norm_([q], 1.0), lambda: ops.grad_norm([q]), lambda: ops.layer_norm(q), lambda: ops.layer_norm_forward(q),
+                 lambda: ops.chain_rows(t, tgt, [t[0]]), lambda: ops.chain_rows_backward(q, t, tgt, [], t, [])):
         with pytest.raises(GqeLibraryError):
             call()
     with pytest.raises(ValueError):
