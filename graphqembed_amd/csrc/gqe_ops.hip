@@ -55,6 +55,7 @@ bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 // softmax cross entropy: join of the splits
 // ------------------------------------------------------------------------------------------------------------------------------
 #define XENT_MAX_SPLIT 1024
+#define XENT_JOIN_BATCH 8
 
 struct XentJoin {
   const float *part_m, *part_l, *part_o, *st;
@@ -63,7 +64,7 @@ struct XentJoin {
   const float* weight;
   const void* table;       // DQ: the target's row; DT: the row itself
   int64_t table_stride;
-  int32_t unit, out_f32, accumulate;
+  int32_t unit, out_f32, accumulate, lanes, pitch;
   float scale;
   float *loss, *lse, *stat;
   XentRec* rec;            // LSE / DQ: the queries as streamed rows of the table's gradient, which this call goes on to
@@ -109,42 +110,126 @@ __device__ __forceinline__ double log2_of(double x) {
   return x > 0.0 ? (double)(e - 1) + (double)log2f((float)(f + f)) : x == 0.0 ? -INFINITY : x;
 }
 
-// One workgroup of WAVES waves per stationary row: the splits' sums brought to one unit and added in a fixed order.  Bound by the
-// latency of n_split rows of partial sums: eight waves share them, 16 bytes a lane, eight of them under way (512 rows of 125 x 512
-// bytes, 33 MB: 10 us; four waves, 4 bytes a lane: 27 us).
-template <bool BF16, int MODE, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
-  __shared__ float ws[MODE == XENT_MODE_LSE ? 1 : XENT_MAX_SPLIT];
-  __shared__ double red[WAVES];
-  __shared__ float redf[WAVES];
-  __shared__ __align__(16) float acc[WAVES + 1][256];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t y = blockIdx.x;
-  float m = XENT_NONE;
-  for (int s = tid; s < p.n_split; s += 64 * WAVES) m = fmaxf(m, p.part_m[(int64_t)s * p.ny + y]);
-  m = wave_max(m);
-  if (WAVES > 1) {
-    if (lane == 0) redf[wave] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, redf[w]);
-  }
-  float half = 0.f, f = 0.f, share = 0.f, g = 0.f;      // half * f: the unit's power in two factors, the sums carry the operands' 2^30
-  int tg = -1;
-  if (MODE != XENT_MODE_DT) {
-    double l = 0.0;
-    for (int s = tid; s < p.n_split; s += 64 * WAVES)
-      l += (double)p.part_l[(int64_t)s * p.ny + y] * (double)exp2f(p.part_m[(int64_t)s * p.ny + y] - m);
-    l = wave_sum_f64(l);
-    if (WAVES > 1) {
-      if (lane == 0) red[wave] = l;
-      __syncthreads();
-      l = 0.0;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) l += red[w];
+// four elements of a row, wherever it begins (those behind column d: zero)
+template <bool BF16>
+__device__ __forceinline__ void row_four(const void* p, int64_t at, int left, float* t) {
+  if (left >= 4) {
+    if (BF16) {
+      const XentU2 u = *(const XentU2*)((const uint16_t*)p + at);
+      t[0] = bf16_lo(u.v[0]); t[1] = bf16_hi(u.v[0]); t[2] = bf16_lo(u.v[1]); t[3] = bf16_hi(u.v[1]);
+    } else {
+      const XentF4 u = *(const XentF4*)((const float*)p + at);
+      t[0] = u.v[0]; t[1] = u.v[1]; t[2] = u.v[2]; t[3] = u.v[3];
     }
-    tg = p.target[y];
-    const bool has = tg >= 0 && tg < p.n_rows;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = i < left ? row_elem<BF16>(p, at + i) : 0.f;
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void put_four(void* p, int64_t at, int left, const float* v, bool accumulate) {
+  if (left >= 4) {
+    if (BF16) {
+      *(XentU2*)((uint16_t*)p + at) = XentU2{{xent_pack_bf16(v[0], v[1]), xent_pack_bf16(v[2], v[3])}};
+    } else {
+      XentF4* q = (XentF4*)((float*)p + at);
+      const XentF4 w = accumulate ? *q : XentF4{{0.f, 0.f, 0.f, 0.f}};
+      *q = XentF4{{accumulate ? w.v[0] + v[0] : v[0], accumulate ? w.v[1] + v[1] : v[1], accumulate ? w.v[2] + v[2] : v[2], accumulate ? w.v[3] + v[3] : v[3]}};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) put_elem<BF16>(p, at + i, v[i], accumulate);
+  }
+}
+
+// The splits' sums of a stationary row, each with its own unit 2^part_m, added in a fixed order.  Bound by latency: a lane takes 16 bytes of
+// a split, `lanes` of them a row, so that a wave has 64 / lanes splits at once and eight times as many under way, and nothing waits for
+// the largest unit: each lane's sums follow a running one of their own and are brought together at the end.  WAVES = 1: a wave per row,
+// four rows a workgroup (few splits, many rows); 16: a workgroup per row.
+template <bool BF16, int MODE, int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
+  constexpr bool LSE = MODE == XENT_MODE_LSE, DT = MODE == XENT_MODE_DT;
+  constexpr int BATCH = XENT_JOIN_BATCH;
+  __shared__ float redm[WAVES];
+  __shared__ double redl[WAVES];
+  __shared__ __align__(16) float acc[WAVES == 1 || LSE ? 1 : WAVES][256];
+  const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
+  const int64_t y = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (WAVES == 1 && y >= p.ny) return;
+  const int lanes = LSE ? 1 : p.lanes, c = 4 * (lane & (lanes - 1)), left = p.d - c;
+  const int at_once = 64 / lanes * WAVES, first = wave * (64 / lanes) + lane / lanes;
+  // the target's row (DQ), the row itself (DT)
+  int tg = -1;
+  if (!DT) tg = p.target[y];
+  const bool has = !DT && tg >= 0 && tg < p.n_rows;
+  const int64_t row = DT ? y : has ? tg : -1;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  if (!LSE && wave == 0 && row >= 0 && (!DT || p.unit) && left > 0) row_four<BF16>(p.table, row * p.table_stride + c, left, t);
+
+  float m = XENT_NONE, v[4] = {0.f, 0.f, 0.f, 0.f};
+  double l = 0.0;
+  for (int s0 = first; s0 < p.n_split; s0 += BATCH * at_once) {
+    float pm[BATCH], pl[BATCH];
+    float4 u[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int64_t at = (int64_t)(s0 + i * at_once) * p.ny + y;
+      const bool in = s0 + i * at_once < p.n_split;
+      pm[i] = in ? p.part_m[at] : XENT_NONE;
+      pl[i] = !DT && in && c == 0 ? p.part_l[at] : 0.f;
+      u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (!LSE && in && left > 0) u[i] = *(const float4*)(p.part_o + at * p.pitch + c);
+    }
+    float now = m;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) now = fmaxf(now, pm[i]);
+    const float w0 = exp2f(m - now);
+    m = now;
+    l *= (double)w0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] *= w0;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float w = exp2f(pm[i] - m);
+      l += (double)pl[i] * (double)w;
+      v[0] = fmaf(w, u[i].x, v[0]); v[1] = fmaf(w, u[i].y, v[1]); v[2] = fmaf(w, u[i].z, v[2]); v[3] = fmaf(w, u[i].w, v[3]);
+    }
+  }
+  {
+    const float top = wave_max(m), w = exp2f(m - top);
+    m = top;
+    if (!DT) l = wave_sum_f64(l * (double)w);
+    if (!LSE) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] *= w;
+      for (int o = lanes; o < 64; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += __shfl_xor(v[k], o);
+    }
+  }
+  if (WAVES > 1) {
+    if (lane == 0) { redm[wave] = m; redl[wave] = l; }
+    if (!LSE && lane < lanes) *(float4*)&acc[wave][c] = make_float4(v[0], v[1], v[2], v[3]);
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, redm[w]);
+    l = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float f = exp2f(redm[w] - m);
+      l += redl[w] * (double)f;
+      if (!LSE) {
+        const float4 u = *(const float4*)&acc[w][c];
+        v[0] = fmaf(f, u.x, v[0]); v[1] = fmaf(f, u.y, v[1]); v[2] = fmaf(f, u.z, v[2]); v[3] = fmaf(f, u.w, v[3]);
+      }
+    }
+  }
+  float half, f, share = 0.f, g = 0.f;      // half * f: the unit's power in two factors, the sums carry the operands' 2^30
+  if (!DT) {
     const double others = (double)m + log2_of(l);           // -inf where the target is the only row
     double lse2 = others, lr = 0.0, loss = 0.0;
     if (has) {
@@ -159,127 +244,73 @@ __global__ __launch_bounds__(64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
       loss = __longlong_as_double(0x7ff8000000000000LL);
     }
     g = has ? (p.weight ? p.weight[y] : 1.f) : 0.f;
-    if (tid == 0) {
+    if (lane == 0) {
       if (p.loss) p.loss[y] = (float)loss;
       if (p.lse) p.lse[y] = (float)(lse2 * 0.6931471805599453);
       p.stat[2 * y] = (float)lse2;
       p.stat[2 * y + 1] = (float)lr;
     }
-    if (p.rec && tid < XENT_TR) {      // (the last row's workgroup: also what fills its tile)
+    if (p.rec && lane < XENT_TR) {      // (the last row: also what fills its tile)
       const int i = (int)(y % XENT_TR), last = y == p.ny - 1 ? XENT_TR - 1 : i;
-      if (tid >= i && tid <= last) {
-        const bool ok = tid == i;
-        const float c = ok ? p.fac[y].x : 1.f;
-        xent_rec_dt(p.rec[y / XENT_TR], tid, ok, c, BF16 ? 0.f : xent_exponent(c), ok ? tg : -1, ok ? (p.weight ? p.weight[y] : 1.f) : 0.f, (float)lse2,
+      if (lane >= i && lane <= last) {
+        const bool ok = lane == i;
+        const float k = ok ? p.fac[y].x : 1.f;
+        xent_rec_dt(p.rec[y / XENT_TR], lane, ok, k, BF16 ? 0.f : xent_exponent(k), ok ? tg : -1, ok ? (p.weight ? p.weight[y] : 1.f) : 0.f, (float)lse2,
                     (float)lr, p.n_rows, p.scale2);
       }
     }
-    if (MODE == XENT_MODE_LSE) return;
-    if (!has) tg = -1;
+    if (LSE) return;
     share = exp2_of(lr);
     half = f = exp2_of(0.5 * ((double)m - lse2));
   } else {
     half = exp2f(0.5f * m);
     f = p.scale * half;
   }
-  for (int s = tid; s < p.n_split; s += 64 * WAVES) ws[s] = exp2f(p.part_m[(int64_t)s * p.ny + y] - m);
-  __syncthreads();
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  const int64_t step = (int64_t)p.ny * p.d;
-  const float* po = p.part_o + y * p.d;
-  const bool vec = (p.d & 3) == 0;
-  if (vec) {                   // d <= 128: two splits at a time, 32 lanes each
-    const int two = p.d <= 128 ? 1 : 0, c = 4 * (two ? lane & 31 : lane);
-    const int first = two ? 2 * wave + (lane >> 5) : wave, stride = two ? 2 * WAVES : WAVES;
-    if (c < p.d) {
-#pragma unroll 8
-      for (int s = first; s < p.n_split; s += stride) {
-        const float w = ws[s];
-        const float4 u = *(const float4*)(po + s * step + c);
-        v[0] = fmaf(w, u.x, v[0]); v[1] = fmaf(w, u.y, v[1]); v[2] = fmaf(w, u.z, v[2]); v[3] = fmaf(w, u.w, v[3]);
-      }
-    }
-    if (two) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], 32);
-    }
-    if (c < 256 && lane * 4 == c) *(float4*)&acc[wave][c] = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-#pragma unroll 4
-    for (int s = wave; s < p.n_split; s += WAVES) {
-      const float w = ws[s];
+  for (int k = 0; k < 4; ++k) v[k] = v[k] * half * f;
+  const bool mine = lane < lanes && left > 0;     // (behind the sums every group of `lanes` holds the row)
+  float rn = 1.f;
+  if (row >= 0 && p.unit) {
+    const float k = xent_pow2(xent_row_scale(wave_max(fmaxf(fmaxf(fabsf(t[0]), fabsf(t[1])), fmaxf(fabsf(t[2]), fabsf(t[3]))))));
+    float ss = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (lane + 64 * c < p.d) v[c] = fmaf(w, po[s * step + lane + 64 * c], v[c]);
-    }
+    for (int i = 0; i < 4; ++i) ss = fmaf(t[i] * k, t[i] * k, ss);
+    rn = xent_rsqrt(wave_sum(lane < lanes ? ss : 0.f)) * k;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[wave][lane + 64 * c] = v[c];
+    for (int i = 0; i < 4; ++i) t[i] *= rn;
   }
-  __syncthreads();
-  if (wave) return;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    v[c] = 0.f;
-    if (lane + 64 * c < p.d) {
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) v[c] += acc[w][lane + 64 * c];
-    }
-    v[c] = v[c] * half * f;
-  }
-  const int64_t row = MODE == XENT_MODE_DT ? y : tg;
-  float t[4] = {0.f, 0.f, 0.f, 0.f}, rn = 1.f;
-  if (row >= 0 && (MODE == XENT_MODE_DQ || p.unit)) {
-    float mx = 0.f;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (lane + 64 * c < p.d) {
-        t[c] = row_elem<BF16>(p.table, row * p.table_stride + lane + 64 * c);
-        mx = fmaxf(mx, fabsf(t[c]));
-      }
-    if (p.unit) {
-      const float k = xent_pow2(xent_row_scale(wave_max(mx)));
-      float ss = 0.f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) ss = fmaf(t[c] * k, t[c] * k, ss);
-      rn = xent_rsqrt(wave_sum(ss)) * k;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) t[c] *= rn;
-    }
-  }
-  if (MODE == XENT_MODE_DQ) {
+  if (!DT) {
     const float gs = g * p.scale;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) v[c] = g != 0.f ? gs * fmaf(-share, t[c], v[c]) : 0.f;
+    for (int i = 0; i < 4; ++i) v[i] = g != 0.f ? gs * fmaf(-share, t[i], v[i]) : 0.f;
   } else if (p.unit) {
     float along = 0.f;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) along = fmaf(t[c], v[c], along);
-    along = wave_sum(along);
+    for (int i = 0; i < 4; ++i) along = fmaf(t[i], v[i], along);
+    along = wave_sum(lane < lanes ? along : 0.f);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) v[c] = (v[c] - t[c] * along) * rn;
+    for (int i = 0; i < 4; ++i) v[i] = (v[i] - t[i] * along) * rn;
   }
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + 64 * c < p.d) {
-      if (p.out_f32) put_elem<false>(p.out, y * p.out_stride + lane + 64 * c, v[c], p.accumulate != 0);
-      else put_elem<BF16>(p.out, y * p.out_stride + lane + 64 * c, v[c], p.accumulate != 0);
-    }
+  if (!mine) return;
+  if (p.out_f32) put_four<false>(p.out, y * p.out_stride + c, left, v, p.accumulate != 0);
+  else put_four<BF16>(p.out, y * p.out_stride + c, left, v, p.accumulate != 0);
 }
 
 struct XentPlan {
   int dk, n_tiles, n_yblk, n_split, per;
 };
 
-// Splits of the streamed axis: enough workgroups to fill the 256 CUs (`slots` of them at once), `least` tiles in each.  The table's
-// gradient takes four at least: below that the join costs more than a split saves.
+// Splits of the streamed axis: enough workgroups to fill the 256 CUs (`slots` of them at once), `least` tiles in each at least.  The table's
+// gradient takes four: below that the join costs more than a split saves (136 queries, 14575 rows of d = 200, 5 tiles: 20 us and a join of
+// 11 us as 4 + 1).
 XentPlan xent_plan(int64_t ny, int64_t nx, int dim, int slots, int least) {
   XentPlan r;
   r.dk = dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
   r.n_tiles = (int)((nx + XENT_TR - 1) / XENT_TR);
   r.n_yblk = (int)((ny + XENT_BM - 1) / XENT_BM);
-  int64_t s = std::max<int64_t>(1, slots / std::max(r.n_yblk, 1));
-  s = std::min<int64_t>(std::min<int64_t>(s, XENT_MAX_SPLIT), std::max(r.n_tiles, 1));
-  r.per = std::max(least, (int)((r.n_tiles + s - 1) / s));
+  int64_t s = std::min<int64_t>(slots / std::max(r.n_yblk, 1), XENT_MAX_SPLIT);
+  s = std::max<int64_t>(1, std::min<int64_t>(s, r.n_tiles / least));
+  r.per = (int)std::max<int64_t>(1, (r.n_tiles + s - 1) / s);
   r.n_split = std::max(1, (r.n_tiles + r.per - 1) / r.per);
   return r;
 }
@@ -305,7 +336,7 @@ XentSpace xent_space(const gqe_xent_args* a, const XentPlan& q, const XentPlan& 
   s.part_l = take(4 * pq);
   s.st = take(first ? 4 * a->n_queries : 0);
   s.stat = take(a->stat ? 0 : 8 * a->n_queries);
-  s.part_o = take(4 * (int64_t)a->dim * std::max(dq ? pq : 0, pt));
+  s.part_o = take(4 * up(a->dim, 4) * std::max(dq ? pq : 0, pt));
   const int64_t n[2] = {a->n_queries, a->n_rows};
   for (int i = 0; i < 2; ++i) {      // (sizes alone decide: room for the image also where the rows turn out to be usable as they lie)
     s.image[i] = take(xent_prepares(a) ? up(n[i], XENT_TR) * q.dk * (a->dtype == GQE_BF16 ? 2 : 4) : 0);
@@ -334,16 +365,21 @@ hipError_t xent_prep(bool bf16, int dk, bool unit, const XentPrep& p, hipStream_
   }
 }
 
-template <int MODE>
+template <int MODE, int WAVES>
 void join_launch(bool bf16, const XentJoin& j, hipStream_t s) {
-  const dim3 grid((unsigned)j.ny);
-  if (j.n_split > (MODE == XENT_MODE_LSE ? 64 : 8)) {      // (losses alone: a wave reads 64 splits at once)
-    if (bf16) gqe_xent_join_kernel<true, MODE, 8><<<grid, dim3(512), 0, s>>>(j);
-    else gqe_xent_join_kernel<false, MODE, 8><<<grid, dim3(512), 0, s>>>(j);
-  } else {
-    if (bf16) gqe_xent_join_kernel<true, MODE, 1><<<grid, dim3(64), 0, s>>>(j);
-    else gqe_xent_join_kernel<false, MODE, 1><<<grid, dim3(64), 0, s>>>(j);
-  }
+  const dim3 grid((unsigned)(WAVES == 1 ? (j.ny + 3) / 4 : j.ny)), block(WAVES == 1 ? 256 : 64 * WAVES);
+  if (bf16) gqe_xent_join_kernel<true, MODE, WAVES><<<grid, block, 0, s>>>(j);
+  else gqe_xent_join_kernel<false, MODE, WAVES><<<grid, block, 0, s>>>(j);
+}
+// More splits than a wave takes in one go (64 / lanes of them, XENT_JOIN_BATCH times): 16 waves a row, or 8 where there are rows for every
+// CU (229 splits of d = 208: 58 rows 12 us against 18, 512 rows of 64 splits 16 us against 11).
+template <int MODE>
+void join_launch(bool bf16, XentJoin j, hipStream_t s) {
+  j.lanes = 1;
+  while (MODE != XENT_MODE_LSE && 4 * j.lanes < j.d) j.lanes *= 2;
+  if (j.n_split * j.lanes <= 64 * XENT_JOIN_BATCH) join_launch<MODE, 1>(bf16, j, s);
+  else if (j.ny > 256) join_launch<MODE, 8>(bf16, j, s);
+  else join_launch<MODE, 16>(bf16, j, s);
 }
 
 // sizes alone: what the workspace depends on
@@ -396,12 +432,10 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
   if (dev.status != hipSuccess) return hip_refuse(dev.status, "softmax_xent");
   hipStream_t stream = (hipStream_t)a->stream;
   char* w = (char*)a->workspace;
-  const int vec = bf16 ? 8 : 4;
-  const bool dvec = a->dim % 8 == 0;
-  const auto rows_vec = [&](const void* ptr, int64_t stride) { return dvec && aligned(ptr, 16) && stride % vec == 0; };
 
   XentPass p = {};
   p.d = a->dim;
+  p.pitch = (int32_t)up(a->dim, 4);
   p.scale2 = (float)((double)a->scale * 1.4426950408889634);
   p.scale = a->scale;
   p.target = a->target;
@@ -413,7 +447,7 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
   p.stat = stat;
   XentJoin j = {};
   j.part_m = p.part_m; j.part_l = p.part_l; j.part_o = p.part_o; j.st = p.st;
-  j.d = a->dim; j.n_rows = (int32_t)V; j.target = a->target; j.weight = a->weight;
+  j.d = a->dim; j.pitch = p.pitch; j.n_rows = (int32_t)V; j.target = a->target; j.weight = a->weight;
   j.table = a->table; j.table_stride = a->table_stride; j.unit = a->normalize ? 1 : 0; j.scale = a->scale;
   const bool unit = a->normalize != 0, dma = xent_prepares(a);
   const char* image[2] = {};
@@ -425,7 +459,7 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     const void* rows[2] = {a->q, a->table};
     const int64_t n[2] = {B, V}, st[2] = {a->q_stride, a->table_stride};
     for (int i = 0; i < 2; ++i) {
-      r.r[i] = XentRows{rows[i], st[i], (int32_t)n[i], a->dim, rows_vec(rows[i], st[i])};
+      r.r[i] = XentRows{rows[i], st[i], (int32_t)n[i], a->dim};
       r.fac[i] = (float2*)(w + sp.fac[i]);
       r.tiles[i] = (int32_t)((n[i] + XENT_TR - 1) / XENT_TR);
       fac[i] = r.fac[i];
@@ -441,8 +475,8 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     if (e != hipSuccess) return hip_refuse(e, "softmax_xent");
   }
   if (first && B) {
-    p.y = a->q; p.y_stride = a->q_stride; p.ny = (int32_t)B; p.y_vec = rows_vec(a->q, a->q_stride);
-    p.x = a->table; p.x_stride = a->table_stride; p.nx = (int32_t)V; p.x_vec = rows_vec(a->table, a->table_stride);
+    p.y = a->q; p.y_stride = a->q_stride; p.ny = (int32_t)B;
+    p.x = a->table; p.x_stride = a->table_stride; p.nx = (int32_t)V;
     p.n_tiles = pq.n_tiles; p.tiles_per_split = pq.per; p.n_split = pq.n_split; p.n_yblk = pq.n_yblk;
     if (dma) {
       p.y_image = image[0]; p.y_fac = fac[0]; p.y_stride = stride[0];
@@ -461,12 +495,11 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     if ((e = hipGetLastError()) != hipSuccess) return hip_refuse(e, "softmax_xent");
   }
   if (dt) {
-    p.y = a->table; p.y_stride = a->table_stride; p.ny = (int32_t)V; p.y_vec = rows_vec(a->table, a->table_stride);
-    p.x = a->q; p.x_stride = a->q_stride; p.nx = (int32_t)B; p.x_vec = rows_vec(a->q, a->q_stride);
+    p.y = a->table; p.y_stride = a->table_stride; p.ny = (int32_t)V;
+    p.x = a->q; p.x_stride = a->q_stride; p.nx = (int32_t)B;
     p.weight = a->weight;
     p.n_tiles = pt.n_tiles; p.tiles_per_split = pt.per; p.n_split = pt.n_split; p.n_yblk = pt.n_yblk;
     p.out = a->dtable; p.out_stride = a->dtable_stride; p.accumulate = a->accumulate;
-    p.out_vec = a->dim % 4 == 0 && aligned(a->dtable, bf16 ? 8 : 16) && a->dtable_stride % 4 == 0;
     if (dma) {
       p.y_image = image[1]; p.y_fac = fac[1]; p.y_stride = stride[1];
       p.x_image = image[0]; p.x_rec = (const XentRec*)(w + sp.rec); p.x_stride = stride[0];

@@ -63,7 +63,7 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
     __builtin_amdgcn_sched_barrier(0);                   \
   } while (0)
 // two waves in a SIMD's 512 registers, where the operands and sums of 32 stationary rows leave room
-#define XENT_TWO (DK <= 64 || (DK <= 128 && (BF16 || DMA || MODE == XENT_MODE_LSE)))
+#define XENT_TWO (DK <= 128)
 #define XENT_NONE (-1.0e30f)   // running maximum before the first term (finite: its difference from -inf is -inf)
 
 enum { XENT_MODE_LSE = 0, XENT_MODE_DQ = 1, XENT_MODE_DT = 2 };
@@ -73,7 +73,6 @@ struct XentPass {
   const void* x;               // streamed rows:   table rows (LSE, DQ), queries (DT)
   int64_t y_stride, x_stride;
   int32_t ny, nx, d;
-  int32_t y_vec, x_vec;        // rows are 16-byte aligned and d is whole vectors
   const char *y_image, *x_image;      // DMA: prepared tiles, or bfloat16 rows (then the strides are not 0)
   const float2* y_fac;         // DMA: factors of the stationary rows
   const struct XentRec* x_rec; // DMA: the streamed rows' part
@@ -86,11 +85,11 @@ struct XentPass {
   const float* stat;           // DT: [queries][2]
   float* part_m;               // [n_split][ny] running maximum (its unit of the sums)
   float* part_l;               // [n_split][ny] LSE / DQ: sum over the other rows in units of 2^part_m
-  float* part_o;               // [n_split][ny][d] (DQ; DT when split)
+  float* part_o;               // [n_split][ny][pitch] (DQ; DT when split)
   float* st;                   // [queries] LSE / DQ: s of the target
   void* out;                   // DT, n_split == 1: dtable
   int64_t out_stride;
-  int32_t out_vec, accumulate;
+  int32_t pitch, accumulate;   // pitch: d up to whole 16 bytes
 };
 
 __device__ __forceinline__ float xent_pow2(int k) { return __int_as_float((k + 127) << 23); }   // -126 <= k <= 127
@@ -140,11 +139,20 @@ __device__ __forceinline__ f32x16 xent_mfma(const XentFrag& a, const XentFrag& b
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
 }
 
-// Rows of a matrix in global memory.
+// Rows of a matrix in global memory, and 16 bytes of them at an element's alignment.
 struct XentRows {
   const void* p;
   int64_t stride;
-  int32_t n, d, vec;
+  int32_t n, d;
+};
+struct __attribute__((packed, aligned(2))) XentU4 {
+  uint32_t v[4];
+};
+struct __attribute__((packed, aligned(4))) XentF4 {
+  float v[4];
+};
+struct __attribute__((packed, aligned(2))) XentU2 {
+  uint32_t v[2];
 };
 
 // Tile of operands, in LDS and (where it is prepared once) in memory alike: each plane is sub-tiles of 32 rows x 128 columns (8 KB) and,
@@ -220,6 +228,7 @@ struct XentStage {
   static constexpr int NCH = DK / 64;          // pieces of 8 elements: piece c of thread t holds columns 64 c + 8 t ..
   uint32_t raw[NCH][BF16 ? 4 : 8];
 
+  // Pieces of 16 bytes wherever rows begin (the memory takes any alignment); a row's last piece element by element where d cuts it.
   __device__ __forceinline__ void load(const XentRows& r, int row, int t8) {
     const bool ok = row < r.n;
     const int64_t off = (int64_t)row * r.stride;
@@ -231,9 +240,9 @@ struct XentStage {
       if (!ok || col >= r.d) continue;
       if (BF16) {
         const uint16_t* q = (const uint16_t*)r.p + off + col;
-        if (r.vec) {
-          const uint4 u = *(const uint4*)q;
-          raw[c][0] = u.x; raw[c][1] = u.y; raw[c][2] = u.z; raw[c][3] = u.w;
+        if (col + 8 <= r.d) {
+          const XentU4 u = *(const XentU4*)q;
+          raw[c][0] = u.v[0]; raw[c][1] = u.v[1]; raw[c][2] = u.v[2]; raw[c][3] = u.v[3];
         } else {
           uint32_t e[8];
 #pragma unroll
@@ -243,11 +252,12 @@ struct XentStage {
         }
       } else {
         const float* q = (const float*)r.p + off + col;
-        if (r.vec) {
+        if (col + 8 <= r.d) {
 #pragma unroll
           for (int i = 0; i < 8; i += 4) {
-            const uint4 u = *(const uint4*)(q + i);
-            raw[c][i] = u.x; raw[c][i + 1] = u.y; raw[c][i + 2] = u.z; raw[c][i + 3] = u.w;
+            const XentF4 u = *(const XentF4*)(q + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) raw[c][i + k] = __float_as_uint(u.v[k]);
           }
         } else {
 #pragma unroll
@@ -457,8 +467,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   const bool active = y0 < p.ny, y_ok = y < p.ny;
   const int tile0 = split * p.tiles_per_split;
   const int tile1 = min(tile0 + p.tiles_per_split, p.n_tiles);
-  const XentRows xr = {p.x, p.x_stride, p.nx, p.d, p.x_vec};
-  const XentRows yr = {p.y, p.y_stride, p.ny, p.d, p.y_vec};
+  const XentRows xr = {p.x, p.x_stride, p.nx, p.d}, yr = {p.y, p.y_stride, p.ny, p.d};
 
   // this thread's places in a tile
   const Tile wr = {xent_full(srow, t8), xent_half(srow, t8)};                            // stage stores
@@ -876,27 +885,29 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
       const int row = 4 * k + trow, col = 64 * c + tcol;
       float4 v = *(const float4*)(turn + row * L::OUT_ROW + tcol);
       if (y0 + row < p.ny && col < p.d) {
-        if (BF16 && last) {
+        const bool whole = col + 4 <= p.d;
+        if (!last) {                             // (columns behind d are zero)
+          *(float4*)(p.part_o + ((int64_t)split * p.ny + y0 + row) * p.pitch + col) = v;
+        } else if (BF16) {
           uint16_t* po = (uint16_t*)p.out + (int64_t)(y0 + row) * p.out_stride + col;
           const uint32_t a = xent_pack_bf16(v.x, v.y), b = xent_pack_bf16(v.z, v.w);
-          if (p.out_vec) {
-            *(uint2*)po = make_uint2(a, b);
+          if (whole) {
+            *(XentU2*)po = XentU2{{a, b}};
           } else {
             po[0] = (uint16_t)a;
             if (col + 1 < p.d) po[1] = (uint16_t)(a >> 16);
             if (col + 2 < p.d) po[2] = (uint16_t)b;
-            if (col + 3 < p.d) po[3] = (uint16_t)(b >> 16);
           }
         } else {
-          float* po = last ? (float*)p.out + (int64_t)(y0 + row) * p.out_stride + col : p.part_o + ((int64_t)split * p.ny + y0 + row) * p.d + col;
-          if (last ? p.out_vec : (p.d & 3) == 0) {
-            if (last && p.accumulate) { const float4 w = *(const float4*)po; v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w; }
-            *(float4*)po = v;
+          float* po = (float*)p.out + (int64_t)(y0 + row) * p.out_stride + col;
+          if (whole) {
+            if (p.accumulate) { const XentF4 w = *(const XentF4*)po; v.x += w.v[0]; v.y += w.v[1]; v.z += w.v[2]; v.w += w.v[3]; }
+            *(XentF4*)po = XentF4{{v.x, v.y, v.z, v.w}};
           } else {
-            const float e4[4] = {v.x, v.y, v.z, v.w};
+            const float e4[3] = {v.x, v.y, v.z};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (col + j < p.d) po[j] = last && p.accumulate ? po[j] + e4[j] : e4[j];
+            for (int j = 0; j < 3; ++j)
+              if (col + j < p.d) po[j] = p.accumulate ? po[j] + e4[j] : e4[j];
           }
         }
       }
