@@ -314,11 +314,12 @@ XentPlan xent_plan(int64_t ny, int64_t nx, int dim, int slots, int least) {
   r.n_split = std::max(1, (r.n_tiles + r.per - 1) / r.per);
   return r;
 }
-int xent_slots(int dim) { return dim <= 128 ? 512 : 256; }
 
 // Operands are prepared (one more pass over the table: read, written, and read again instead of it) where more than one block of
 // queries would convert the same rows again; up to XENT_BM queries the passes are bound by memory and convert as they go.
 bool xent_prepares(const gqe_xent_args* a) { return a->n_queries > XENT_BM; }
+// workgroups at once: two a CU where the kernels' registers allow it (XENT_TWO)
+int xent_slots(const gqe_xent_args* a) { return a->dim <= 128 || (a->dtype == GQE_BF16 && a->dim <= 192 && xent_prepares(a)) ? 512 : 256; }
 // bfloat16 rows that are operands as they lie: whole tiles wide, 16-byte pieces
 bool xent_as_is(bool bf16, int dk, int dim, const void* ptr, int64_t stride) { return bf16 && dk == dim && aligned(ptr, 16) && stride % 8 == 0 && stride < (1 << 25); }
 
@@ -371,13 +372,14 @@ void join_launch(bool bf16, const XentJoin& j, hipStream_t s) {
   if (bf16) gqe_xent_join_kernel<true, MODE, WAVES><<<grid, block, 0, s>>>(j);
   else gqe_xent_join_kernel<false, MODE, WAVES><<<grid, block, 0, s>>>(j);
 }
-// More splits than a wave takes in one go (64 / lanes of them, XENT_JOIN_BATCH times): 16 waves a row, or 8 where there are rows for every
-// CU (229 splits of d = 208: 58 rows 12 us against 18, 512 rows of 64 splits 16 us against 11).
+// A wave a row where it takes the splits in one go (64 / lanes of them, XENT_JOIN_BATCH times) or rows are many (4608 rows of 14 splits of
+// d = 192: eight waves 42 us); else 16, or 8 where there are rows for every CU (229 splits of d = 208: 58 rows 12 us against 18; 512
+// rows of 64 splits 16 us against 11).
 template <int MODE>
 void join_launch(bool bf16, XentJoin j, hipStream_t s) {
   j.lanes = 1;
   while (MODE != XENT_MODE_LSE && 4 * j.lanes < j.d) j.lanes *= 2;
-  if (j.n_split * j.lanes <= 64 * XENT_JOIN_BATCH) join_launch<MODE, 1>(bf16, j, s);
+  if (j.n_split * j.lanes <= 64 * XENT_JOIN_BATCH || j.ny > 2048) join_launch<MODE, 1>(bf16, j, s);
   else if (j.ny > 256) join_launch<MODE, 8>(bf16, j, s);
   else join_launch<MODE, 16>(bf16, j, s);
 }
@@ -402,8 +404,8 @@ const char* gqe_ops_last_error(void) { return g_ops_error.c_str(); }
 int64_t gqe_softmax_xent_workspace(const gqe_xent_args* a) {
   const int rc = xent_check_sizes(a);
   if (rc) return rc;
-  const XentPlan q = xent_plan(a->n_queries, a->n_rows, a->dim, xent_slots(a->dim), 1);
-  const XentPlan t = xent_plan(a->n_rows, a->n_queries, a->dim, xent_slots(a->dim), 4);
+  const XentPlan q = xent_plan(a->n_queries, a->n_rows, a->dim, xent_slots(a), 1);
+  const XentPlan t = xent_plan(a->n_rows, a->n_queries, a->dim, xent_slots(a), 4);
   return std::max<int64_t>(256, xent_space(a, q, t).total);
 }
 
@@ -424,7 +426,7 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     return refuse(GQE_ERR_ARG, "softmax_xent: a row stride is smaller than dim %d", a->dim);
   if (!aligned(a->q, esize) || !aligned(a->table, esize) || !aligned(a->dq, a->dq_f32 ? 4 : esize) || !aligned(a->dtable, esize))
     return refuse(GQE_ERR_ARG, "softmax_xent: a pointer is not aligned to its element");
-  const XentPlan pq = xent_plan(B, V, a->dim, xent_slots(a->dim), 1), pt = xent_plan(V, B, a->dim, xent_slots(a->dim), 4);
+  const XentPlan pq = xent_plan(B, V, a->dim, xent_slots(a), 1), pt = xent_plan(V, B, a->dim, xent_slots(a), 4);
   const XentSpace sp = xent_space(a, pq, pt);
   if (a->workspace_bytes < sp.total || (sp.total && (!a->workspace || !aligned(a->workspace, 256))))
     return refuse(GQE_ERR_WORKSPACE, "softmax_xent: needs %lld workspace bytes, 256-byte aligned; got %lld", (long long)sp.total, (long long)a->workspace_bytes);

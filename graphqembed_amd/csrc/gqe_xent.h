@@ -63,7 +63,7 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
     __builtin_amdgcn_sched_barrier(0);                   \
   } while (0)
 // two waves in a SIMD's 512 registers, where the operands and sums of 32 stationary rows leave room
-#define XENT_TWO (DK <= 128)
+#define XENT_TWO (DK <= 128 || (BF16 && DMA && DK <= 192))
 #define XENT_NONE (-1.0e30f)   // running maximum before the first term (finite: its difference from -inf is -inf)
 
 enum { XENT_MODE_LSE = 0, XENT_MODE_DQ = 1, XENT_MODE_DT = 2 };
@@ -475,54 +475,6 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   const int orow = 4 * h + ((lane & 15) >> 2), opiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
   const Tile ro = {xent_full(orow, opiece) + 8 * (lane & 1), xent_half(orow, opiece) + 8 * (lane & 1)};      // second product, 32 columns
 
-  // stationary rows -> operand registers, through LDS
-  XentFrag yf[PL][KS];
-  float cy = 1.f;
-  const auto take = [&](const char* tile) {
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int q = 0; q < PL; ++q) *(uint4*)yf[q][ks].u = *(const uint4*)(tile + rs.at(ks >> 2, 32 * (ks & 3)) + q * L::PLANE);
-  };
-  if (DMA) {                                     // two tiles at a time
-    const XentDma<BF16, DK> dy = {p.y_image, p.y_stride ? 64 * p.y_stride : (int64_t)L::TILE, 2 * p.y_stride, p.ny};
-#pragma unroll
-    for (int w = 0; w < 4; w += 2) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (yblk * XENT_BM + 32 * (w + i) < p.ny) dy.load(yblk * (XENT_BM / 32) + w + i, lds.tile + i * L::TILE, wave, lane);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (wave >> 1 == w >> 1) take(lds.tile + (wave & 1) * L::TILE);
-      __syncthreads();
-    }
-    if (y_ok) {
-      const float2 f = p.y_fac[y];
-      cy = f.x;
-      if (IS_DT && h == 0) lds.rn[32 * wave + n] = f.y;
-    }
-  } else {                                       // 32 rows (a wave's) at a time: whole rows are read, and converted once
-    StageY st[2];
-#pragma unroll
-    for (int w = 0; w < 2; ++w) st[w].load(yr, yblk * XENT_BM + 32 * w + srow, t8);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      st[w & 1].store(lds.tile + (w & 1) * L::TILE, wr);
-      const float c = st[w & 1].cs, r = st[w & 1].rn;
-      if (w < 2) st[w & 1].load(yr, yblk * XENT_BM + 32 * (w + 2) + srow, t8);
-      if (t8 == 0) { lds.rec[w & 1].v[0][srow] = c; lds.rn[32 * w + srow] = r; }
-      __syncthreads();
-      if (wave == w) {
-        take(lds.tile + (w & 1) * L::TILE);
-        cy = lds.rec[w & 1].v[0][n];
-      }
-    }
-    __syncthreads();
-  }
-  if (!IS_DT) cy *= p.scale2;
-  int tgt = -1;
-  if (!IS_DT && y_ok) tgt = p.target[y];
-
   // Streamed rows.  DMA: tiles t + 2 and t + 3 are under way while tile t + 1 is multiplied and tile t summed; the vector unit has
   // nothing to do with them.  Otherwise: loads of tile t + 3 are under way while tile t + 2 is converted and stored.
   Stage stage;
@@ -554,6 +506,61 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
       }
     }
   };
+
+  // stationary rows -> operand registers, through LDS.  (DMA: the first streamed tile is asked for before them, into the one place that
+  // they do not pass through, what belongs to the rows likewise: small problems are a chain of latencies.)
+  XentFrag yf[PL][KS];
+  float cy = 1.f, ry = 0.f;
+  int tgt = -1;
+  if (!IS_DT && y_ok) tgt = p.target[y];
+  constexpr int FIRST = DMA && OUT ? L::TILES - 1 : 0;       // the first streamed tile's place
+  if (DMA) {
+    if (y_ok) {
+      const float2 f = p.y_fac[y];
+      cy = f.x;
+      ry = f.y;
+    }
+    if (OUT && tile0 < tile1) load(tile0, FIRST, 0);
+  }
+  const auto take = [&](const char* tile) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int q = 0; q < PL; ++q) *(uint4*)yf[q][ks].u = *(const uint4*)(tile + rs.at(ks >> 2, 32 * (ks & 3)) + q * L::PLANE);
+  };
+  if (DMA) {                                     // two tiles at a time
+    const XentDma<BF16, DK> dy = {p.y_image, p.y_stride ? 64 * p.y_stride : (int64_t)L::TILE, 2 * p.y_stride, p.ny};
+#pragma unroll
+    for (int w = 0; w < 4; w += 2) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (yblk * XENT_BM + 32 * (w + i) < p.ny) dy.load(yblk * (XENT_BM / 32) + w + i, lds.tile + i * L::TILE, wave, lane);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (wave >> 1 == w >> 1) take(lds.tile + (wave & 1) * L::TILE);
+      __syncthreads();
+    }
+    if (IS_DT && h == 0) lds.rn[32 * wave + n] = ry;
+  } else {                                       // 32 rows (a wave's) at a time: whole rows are read, and converted once
+    StageY st[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) st[w].load(yr, yblk * XENT_BM + 32 * w + srow, t8);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      st[w & 1].store(lds.tile + (w & 1) * L::TILE, wr);
+      const float c = st[w & 1].cs, r = st[w & 1].rn;
+      if (w < 2) st[w & 1].load(yr, yblk * XENT_BM + 32 * (w + 2) + srow, t8);
+      if (t8 == 0) { lds.rec[w & 1].v[0][srow] = c; lds.rn[32 * w + srow] = r; }
+      __syncthreads();
+      if (wave == w) {
+        take(lds.tile + (w & 1) * L::TILE);
+        cy = lds.rec[w & 1].v[0][n];
+      }
+    }
+    __syncthreads();
+  }
+  if (!IS_DT) cy *= p.scale2;
+
   // DMA: the next two tiles have arrived; those asked for behind them may be under way.  (Every step asks for one tile, the last ones for
   // the last tile again, into a place that nobody reads: the count is always the same.)
   const auto arrived = [&]() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"((L::DIST - 2) * IN_FLIGHT) : "memory"); };
@@ -584,7 +591,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   // their own, or go before the large ones: every addition rounds at the sum's size, and theirs is 2^-11 of the large one's.  (d <= 128
   // runs two waves in 512 registers: there one sum, and the high halves are read twice.)
   constexpr bool APART = !BF16 && DK > 128;
-  constexpr int AHEAD = BF16 ? (KS < 6 ? KS : 6) : APART ? 3 : 2;
+  constexpr int AHEAD = BF16 ? (DK == 192 ? 3 : KS < 6 ? KS : 6) : APART ? 3 : 2;
   f32x16 s;
   XentFrag fa[AHEAD + 1], fl[AHEAD + 1];
   const auto fetch = [&](const Tile& rt, int ks, bool low) {
@@ -617,11 +624,9 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if (ks + AHEAD < KS) fetch(rt, ks + AHEAD, APART);
+      if (APART) small = xent_mfma<BF16>(fa[ks % (AHEAD + 1)], yf[PL - 1][ks], small);
       acc = xent_mfma<BF16>(fa[ks % (AHEAD + 1)], yf[0][ks], acc);
-      if (APART) {
-        small = xent_mfma<BF16>(fa[ks % (AHEAD + 1)], yf[PL - 1][ks], small);
-        small = xent_mfma<BF16>(fl[ks % (AHEAD + 1)], yf[0][ks], small);
-      }
+      if (APART) small = xent_mfma<BF16>(fl[ks % (AHEAD + 1)], yf[0][ks], small);
       if (BF16 || APART) between(ks);
       XENT_MIX(APART ? 3 : 1);
     }
@@ -643,9 +648,8 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   if (tile0 < tile1) {
     if (DMA) {
 #pragma unroll
-      for (int i = 0; i < L::DIST; ++i)
-        load(min(tile0 + i, tile1 - 1), i, i);
-      arrived();
+      for (int i = OUT ? 1 : 0; i < L::DIST; ++i) load(min(tile0 + i, tile1 - 1), (FIRST + i) % L::TILES, i);
+      if (!OUT) arrived();
     } else {
       load(tile0, 0, 0);
       stage.store(lds.tile, wr);
@@ -657,17 +661,21 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
       }
       if (tile0 + 2 < tile1) load(tile0 + 2, 0, 0);
     }
-    __syncthreads();
+    if (!DMA || !OUT) __syncthreads();           // (else: the first tile came with the stationary rows)
     if (active) {
-      product(0, [](int) {});
+      product(FIRST, [](int) {});
 #pragma unroll
       for (int q = 0; q < 4; ++q) exponents(q, 0);
     }
     if (!OUT && !DMA) __syncthreads();           // two tiles: the first one's place is taken next
+    if (DMA && OUT) {
+      arrived();
+      __syncthreads();
+    }
   }
   int mark = 0x7fffffff;                         // DT: target and sign of the next tile's row n
   if (IS_DT && tile0 < tile1) mark = __float_as_int(lds.rec[0].v[3][n]);
-  int tb = 0, ab = 0;                            // places of tile t: tile modulo TILES, its rows' part modulo RECS
+  int tb = FIRST, ab = 0;                        // places of tile t: tile modulo TILES, its rows' part modulo RECS
   for (int t = tile0; t < tile1; ++t) {
     const int tb1 = tb + 1 == L::TILES ? 0 : tb + 1, tb2 = tb1 + 1 == L::TILES ? 0 : tb1 + 1;
     const int ab1 = ab + 1 == L::RECS ? 0 : ab + 1, ab2 = ab1 + 1 == L::RECS ? 0 : ab1 + 1;
@@ -682,14 +690,14 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         const unsigned at = (unsigned)(tgt - t * XENT_TR);
         found = __any(at < XENT_TR);
         if (found) {
+          float own = 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int row = 8 * (r >> 2) + 4 * h + (r & 3);
-            if ((int)at == row) {
-              p.st[y] = s[r] * (lds.rec[ab].v[0][row] * cy);
-              e[r] = -INFINITY;
-            }
+            const bool hit = (int)at == 8 * (r >> 2) + 4 * h + (r & 3);
+            own = hit ? s[r] : own;
+            e[r] = hit ? -INFINITY : e[r];
           }
+          if (at < XENT_TR && (int)(at >> 2 & 1) == h) p.st[y] = own * (lds.rec[ab].v[0][at] * cy);
         }
       } else {
         const unsigned below = (unsigned)__ballot(mark < 0) >> 4 * h;      // bit 8 q + i: register 4 q + i
@@ -697,11 +705,14 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         found = __any((unsigned)((mark & 0x7fffffff) - y0) < 32u);
         if (found) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int row = 8 * (r >> 2) + 4 * h + (r & 3);
-            if ((__float_as_int(lds.rec[ab].v[3][row]) & 0x7fffffff) == y) {
-              e[r] = lds.rec[ab].v[2][row];
-              neg ^= 1u << r;
+          for (int q = 0; q < 4; ++q) {
+            const float4 own = *(const float4*)&lds.rec[ab].v[2][8 * q + 4 * h], who = *(const float4*)&lds.rec[ab].v[3][8 * q + 4 * h];
+            const float o4[4] = {own.x, own.y, own.z, own.w}, w4[4] = {who.x, who.y, who.z, who.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const bool hit = (__float_as_int(w4[k]) & 0x7fffffff) == y;
+              e[4 * q + k] = hit ? o4[k] : e[4 * q + k];
+              neg ^= hit ? 1u << (4 * q + k) : 0u;
             }
           }
         }
@@ -749,7 +760,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
       };
       typedef __attribute__((address_space(3))) s16x4* lp;
       const Tile rt2 = ro.plus(tb * L::TILE);
-      constexpr int NS = 2 * DT, AH = BF16 ? (NS < 4 ? NS : 4) : 2;
+      constexpr int NS = 2 * DT, AH = BF16 ? (DK == 192 ? 3 : NS < 4 ? NS : 4) : 2;
       XentFrag oa[OUT ? AH + 1 : 1], ol[OUT ? AH + 1 : 1];
       const auto fetch2 = [&](int j) {
         const int sk = j / DT, i = j % DT, chunk = i >> 1, rows = (chunk >> 1 < Tile::FULL ? 256 : 128);
@@ -770,6 +781,9 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
             if (r * KS / 16 == ks) exponential(r);
         });
       } else {
+        // (opaque: else the compiler moves what both branches compute, the exponentials, to before the matrix instructions)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) asm volatile("" : "+v"(e[r]));
 #pragma unroll
         for (int r = 0; r < 16; ++r) exponential(r);
       }
