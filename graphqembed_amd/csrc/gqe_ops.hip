@@ -300,9 +300,7 @@ struct XentPlan {
   int dk, n_tiles, n_yblk, n_split, per;
 };
 
-// Splits of the streamed axis: enough workgroups to fill the 256 CUs (`slots` of them at once), `least` tiles in each at least.  The table's
-// gradient takes four: below that the join costs more than a split saves (136 queries, 14575 rows of d = 200, 5 tiles: 20 us and a join of
-// 11 us as 4 + 1).
+// Splits of the streamed axis: enough workgroups to fill the 256 CUs (`slots` of them at once), `least` tiles in each at least.
 XentPlan xent_plan(int64_t ny, int64_t nx, int dim, int slots, int least) {
   XentPlan r;
   r.dk = dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
@@ -320,6 +318,16 @@ XentPlan xent_plan(int64_t ny, int64_t nx, int dim, int slots, int least) {
 bool xent_prepares(const gqe_xent_args* a) { return a->n_queries > XENT_BM; }
 // workgroups at once: two a CU where the kernels' registers allow it (XENT_TWO)
 int xent_slots(const gqe_xent_args* a) { return a->dim <= 128 || (a->dtype == GQE_BF16 && a->dim <= 192 && xent_prepares(a)) ? 512 : 256; }
+XentPlan xent_plan_queries(const gqe_xent_args* a) { return xent_plan(a->n_queries, a->n_rows, a->dim, xent_slots(a), 1); }
+// The table's gradient takes four tiles of queries at least: below that the join costs more than a split saves (136 queries, 14575 rows of
+// d = 200, 5 tiles: 20 us, and a join of 11 us as 4 + 1).  Where float32 rows of d > 64 are converted on the way a tile takes 3 to 8 us, and
+// with three or four of them and few rows to join each goes by itself (100 queries, 1000 rows of d = 128: 20 us, apart 12 + 4; d = 64: 13
+// us, apart 10 + 5).
+XentPlan xent_plan_table(const gqe_xent_args* a) {
+  const int64_t blocks = (a->n_rows + XENT_BM - 1) / XENT_BM, tiles = (a->n_queries + XENT_TR - 1) / XENT_TR;
+  const bool apart = a->dtype == GQE_F32 && a->dim > 64 && !xent_prepares(a) && tiles >= 3 && blocks * tiles <= 128;
+  return xent_plan(a->n_rows, a->n_queries, a->dim, xent_slots(a), apart ? 1 : 4);
+}
 // bfloat16 rows that are operands as they lie: whole tiles wide, 16-byte pieces
 bool xent_as_is(bool bf16, int dk, int dim, const void* ptr, int64_t stride) { return bf16 && dk == dim && aligned(ptr, 16) && stride % 8 == 0 && stride < (1 << 25); }
 
@@ -404,8 +412,7 @@ const char* gqe_ops_last_error(void) { return g_ops_error.c_str(); }
 int64_t gqe_softmax_xent_workspace(const gqe_xent_args* a) {
   const int rc = xent_check_sizes(a);
   if (rc) return rc;
-  const XentPlan q = xent_plan(a->n_queries, a->n_rows, a->dim, xent_slots(a), 1);
-  const XentPlan t = xent_plan(a->n_rows, a->n_queries, a->dim, xent_slots(a), 4);
+  const XentPlan q = xent_plan_queries(a), t = xent_plan_table(a);
   return std::max<int64_t>(256, xent_space(a, q, t).total);
 }
 
@@ -426,7 +433,7 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
     return refuse(GQE_ERR_ARG, "softmax_xent: a row stride is smaller than dim %d", a->dim);
   if (!aligned(a->q, esize) || !aligned(a->table, esize) || !aligned(a->dq, a->dq_f32 ? 4 : esize) || !aligned(a->dtable, esize))
     return refuse(GQE_ERR_ARG, "softmax_xent: a pointer is not aligned to its element");
-  const XentPlan pq = xent_plan(B, V, a->dim, xent_slots(a), 1), pt = xent_plan(V, B, a->dim, xent_slots(a), 4);
+  const XentPlan pq = xent_plan_queries(a), pt = xent_plan_table(a);
   const XentSpace sp = xent_space(a, pq, pt);
   if (a->workspace_bytes < sp.total || (sp.total && (!a->workspace || !aligned(a->workspace, 256))))
     return refuse(GQE_ERR_WORKSPACE, "softmax_xent: needs %lld workspace bytes, 256-byte aligned; got %lld", (long long)sp.total, (long long)a->workspace_bytes);
