@@ -39,13 +39,9 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 
 #define XENT_BM 128            // stationary rows of a workgroup: 32 for each of its four waves
 #define XENT_TR 32             // streamed rows of an LDS tile
-// closes a step of n matrix instructions: LDS reads first, then matrix instructions with vector work between them
-#ifndef XENT_V
+// closes a step of n matrix instructions: LDS reads first, then matrix instructions with vector work between them (4 to 7 instructions
+// after each: within 1 %)
 #define XENT_V 5
-#endif
-#ifndef X_DIST
-#define X_DIST 2
-#endif
 #define XENT_GROUP(mask, n) __builtin_amdgcn_sched_group_barrier(mask, n, 0)
 #define XENT_MIX(n)                                      \
   do {                                                   \
@@ -211,7 +207,7 @@ struct XentLds {
   static constexpr int PLANES = BF16 ? 1 : 2;
   static constexpr int PLANE = XentTile<DK>::PLANE;
   static constexpr int TILE = PLANES * PLANE;
-  static constexpr int DIST = DMA ? X_DIST : 2;                       // tile t + DIST is asked for while tile t is summed
+  static constexpr int DIST = 2;                                      // tile t + DIST is asked for while tile t is summed (3: no faster)
   static constexpr int TILES = (MODE == XENT_MODE_LSE ? 0 : 1) + DIST;
   static constexpr int RECS = DIST + 1;
   static constexpr int OUT_ROW = 68;                                  // floats of a row of the outputs' turn (64 columns at a time)
@@ -475,40 +471,42 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   const int orow = 4 * h + ((lane & 15) >> 2), opiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
   const Tile ro = {xent_full(orow, opiece) + 8 * (lane & 1), xent_half(orow, opiece) + 8 * (lane & 1)};      // second product, 32 columns
 
-  // Streamed rows.  DMA: tiles t + 2 and t + 3 are under way while tile t + 1 is multiplied and tile t summed; the vector unit has
-  // nothing to do with them.  Otherwise: loads of tile t + 3 are under way while tile t + 2 is converted and stored.
-  Stage stage;
+  // Streamed rows.  DMA: tile t + 2 is under way while tile t + 1 is multiplied and tile t summed; the vector unit has nothing to do with
+  // it.  Otherwise: loads of tile t + 3 are under way while tile t + 2 is converted and stored.
+  struct Feed {
+    Stage st;
+    float g, lse2, lr;        // DT: weight and statistics of this thread's query
+    int target;
+  } feed;
   const XentDma<BF16, DK> dx = {p.x_image, p.x_stride ? 64 * p.x_stride : (int64_t)L::TILE, 2 * p.x_stride, p.nx};
   constexpr int IN_FLIGHT = XentDma<BF16, DK>::N + 1;      // direct loads of a tile, per wave
-  float xg = 0.f, xl = 0.f, xs = 0.f;
-  int xt = -1;
   // DMA: piece i of IN_FLIGHT of tile t; the last one is the rows' part: 512 bytes, each half by two waves (all have as many under way)
   const auto load_piece = [&](int i, int t, int tb, int ab) {
     if (i < IN_FLIGHT - 1) dx.piece(i, t, lds.tile + tb * L::TILE, wave, lane);
     else xent_dma4((const char*)(p.x_rec + t), 256 * (wave & 1) + 4 * lane, xent_lds_addr((char*)&lds.rec[ab] + 256 * (wave & 1)));
   };
   const auto load = [&](int t, int tb, int ab) {
-    if (DMA) {
 #pragma unroll
-      for (int i = 0; i < IN_FLIGHT; ++i) load_piece(i, t, tb, ab);
-      return;
-    }
+    for (int i = 0; i < IN_FLIGHT; ++i) load_piece(i, t, tb, ab);
+  };
+  const auto load_rows = [&](Feed& f, int t) {
     const int x = t * XENT_TR + srow;
-    stage.load(xr, x, t8);
+    f.st.load(xr, x, t8);
     if (IS_DT) {
-      xg = xl = xs = 0.f;
-      xt = -1;
+      f.g = f.lse2 = f.lr = 0.f;
+      f.target = -1;
       if (x < p.nx) {
-        xt = p.target[x];
-        xg = p.weight ? p.weight[x] : 1.f;
-        xl = p.stat[2 * (int64_t)x];
-        xs = p.stat[2 * (int64_t)x + 1];
+        f.target = p.target[x];
+        f.g = p.weight ? p.weight[x] : 1.f;
+        f.lse2 = p.stat[2 * (int64_t)x];
+        f.lr = p.stat[2 * (int64_t)x + 1];
       }
     }
   };
 
-  // stationary rows -> operand registers, through LDS.  (DMA: the first streamed tile is asked for before them, into the one place that
-  // they do not pass through, what belongs to the rows likewise: small problems are a chain of latencies.)
+  // stationary rows -> operand registers, through LDS.  Everything that can be is asked for at once, for small problems are a chain of
+  // latencies: the first streamed tiles (DMA: the first, into the one place that the stationary rows do not pass through), all of the
+  // stationary rows (DMA: two tiles at a time), and what belongs to them.
   XentFrag yf[PL][KS];
   float cy = 1.f, ry = 0.f;
   int tgt = -1;
@@ -521,6 +519,11 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
       ry = f.y;
     }
     if (OUT && tile0 < tile1) load(tile0, FIRST, 0);
+  }
+  Feed second;
+  if (!DMA) {
+    if (tile0 < tile1) load_rows(feed, tile0);
+    if (tile0 + 1 < tile1) load_rows(second, tile0 + 1);
   }
   const auto take = [&](const char* tile) {
 #pragma unroll
@@ -542,15 +545,14 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
     }
     if (IS_DT && h == 0) lds.rn[32 * wave + n] = ry;
   } else {                                       // 32 rows (a wave's) at a time: whole rows are read, and converted once
-    StageY st[2];
+    StageY st[4];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) st[w].load(yr, yblk * XENT_BM + 32 * w + srow, t8);
+    for (int w = 0; w < 4; ++w) st[w].load(yr, yblk * XENT_BM + 32 * w + srow, t8);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      st[w & 1].store(lds.tile + (w & 1) * L::TILE, wr);
-      const float c = st[w & 1].cs, r = st[w & 1].rn;
-      if (w < 2) st[w & 1].load(yr, yblk * XENT_BM + 32 * (w + 2) + srow, t8);
-      if (t8 == 0) { lds.rec[w & 1].v[0][srow] = c; lds.rn[32 * w + srow] = r; }
+      if (yblk * XENT_BM + 32 * w >= p.ny) break;
+      st[w].store(lds.tile + (w & 1) * L::TILE, wr);
+      if (t8 == 0) { lds.rec[w & 1].v[0][srow] = st[w].cs; lds.rn[32 * w + srow] = st[w].rn; }
       __syncthreads();
       if (wave == w) {
         take(lds.tile + (w & 1) * L::TILE);
@@ -561,16 +563,15 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   }
   if (!IS_DT) cy *= p.scale2;
 
-  // DMA: the next two tiles have arrived; those asked for behind them may be under way.  (Every step asks for one tile, the last ones for
-  // the last tile again, into a place that nobody reads: the count is always the same.)
-  const auto arrived = [&]() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"((L::DIST - 2) * IN_FLIGHT) : "memory"); };
-  const auto factors = [&](int t, int ab) {       // (not DMA) behind the tile's operands: its rows' part
-    const float c = stage.cs;
+  // DMA: what this wave asked for has arrived (everyone's: behind the barrier that follows)
+  const auto arrived = [&]() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
+  const auto factors = [&](const Feed& f, int t, int ab) {       // (not DMA) behind the tile's operands: its rows' part
+    const float c = f.st.cs;
     const bool ok = t * XENT_TR + srow < p.nx;
     XentRec& r = lds.rec[ab];
-    float lam = BF16 ? 0.f : (float)-stage.k;
+    float lam = BF16 ? 0.f : (float)-f.st.k;
     if (IS_DT) {
-      xent_rec_dt(r, srow, ok, c, lam, xt, xg, xl, xs, p.ny, p.scale2);
+      xent_rec_dt(r, srow, ok, c, lam, f.target, f.g, f.lse2, f.lr, p.ny, p.scale2);
     } else {
       if (BF16 && UNIT) lam = c > 0.f ? __builtin_amdgcn_logf(c) : 0.f;
       r.v[0][srow] = c;
@@ -648,18 +649,17 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
   if (tile0 < tile1) {
     if (DMA) {
 #pragma unroll
-      for (int i = OUT ? 1 : 0; i < L::DIST; ++i) load(min(tile0 + i, tile1 - 1), (FIRST + i) % L::TILES, i);
+      for (int i = OUT ? 1 : 0; i < L::DIST; ++i)
+        if (tile0 + i < tile1) load(tile0 + i, (FIRST + i) % L::TILES, i);
       if (!OUT) arrived();
     } else {
-      load(tile0, 0, 0);
-      stage.store(lds.tile, wr);
-      factors(tile0, 0);
+      feed.st.store(lds.tile, wr);
+      factors(feed, tile0, 0);
+      if (tile0 + 2 < tile1) load_rows(feed, tile0 + 2);
       if (tile0 + 1 < tile1) {
-        load(tile0 + 1, 0, 0);
-        stage.store(lds.tile + L::TILE, wr);
-        factors(tile0 + 1, 1);
+        second.st.store(lds.tile + L::TILE, wr);
+        factors(second, tile0 + 1, 1);
       }
-      if (tile0 + 2 < tile1) load(tile0 + 2, 0, 0);
     }
     if (!DMA || !OUT) __syncthreads();           // (else: the first tile came with the stationary rows)
     if (active) {
@@ -683,7 +683,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
     const bool more = t + 1 < tile1;
     // DMA: tile t + DIST goes into the place before tile t's, last read by the step before this one (LSE: into tile t's own, its product
     // is done).  Asked for in one go: spread over the steps of the first product it took 4 % longer.
-    if (DMA && more) load(min(t + L::DIST, tile1 - 1), OUT ? (tb == 0 ? L::TILES - 1 : tb - 1) : tb, ab == 0 ? L::RECS - 1 : ab - 1);
+    if (DMA && t + L::DIST < tile1) load(t + L::DIST, OUT ? (tb == 0 ? L::TILES - 1 : tb - 1) : tb, ab == 0 ? L::RECS - 1 : ab - 1);
     if (active) {
       bool found;                                // a target in this tile: its entry is changed, the largest is taken again
       if (!IS_DT) {
@@ -804,7 +804,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
             o[i] = xent_mfma<BF16>(oa[j % (AH + 1)], pf[PL - 1][sk], o[i]);
             o[i] = xent_mfma<BF16>(ol[j % (AH + 1)], pf[0][sk], o[i]);
           }
-          if (!DMA) stage.step(j, lds.tile + tb2 * L::TILE, wr);
+          if (!DMA) feed.st.step(j, lds.tile + tb2 * L::TILE, wr);
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (q * NS / 4 == j) exponents(q, ab1);
@@ -813,24 +813,20 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         }
       }
     }
-    if (!DMA && (!OUT || !active)) stage.store(lds.tile + tb2 * L::TILE, wr);
+    if (!DMA && (!OUT || !active)) feed.st.store(lds.tile + tb2 * L::TILE, wr);
     if (!OUT && active) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) exponents(q, ab1);
     }
     if (!DMA) {
-      factors(t + 2, ab2);
-      if (t + 3 < tile1) load(t + 3, 0, 0);
+      factors(feed, t + 2, ab2);
+      if (t + 3 < tile1) load_rows(feed, t + 3);
     } else {
       arrived();
     }
     __syncthreads();
     tb = tb1;
     ab = ab1;
-  }
-  if (DMA) {                                     // LDS is used again below
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
   }
   if (!active) return;
   if (!IS_DT) l += __shfl_xor(l, 32);
