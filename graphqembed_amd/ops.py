@@ -107,9 +107,10 @@ def _on_gpu(what, *tensors):
     """Index of the HIP device that all tensors are on."""
     index = None
     for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise ValueError("%s: expected a tensor, got %s" % (what, type(t).__name__))
-        i = t.get_device() if t.is_cuda else -1
+        try:
+            i = t.get_device() if t.is_cuda else -1
+        except AttributeError:
+            raise ValueError("%s: expected a tensor, got %s" % (what, type(t).__name__)) from None
         if i < 0:
             raise GqeLibraryError("%s: the operators run on an MI355X only (got a tensor on %s; there is no CPU fallback)" % (what, t.device))
         if index is None:
@@ -171,7 +172,7 @@ def _xent(what, phase, q, table, target, scale, normalize, weight=None, loss=Non
             raise ValueError("%s: weight is float32 [%d], got %s %s" % (what, n, weight.dtype, tuple(weight.shape)))
         weight = weight.contiguous()
     need = _xent_space(phase, dtype, d, n, rows, stat is not None)
-    space = torch.empty(need, dtype=torch.uint8, device=q.device)
+    space = q.new_empty(need, dtype=torch.uint8)
     _check(library().gqe_softmax_xent(_XENT.pack(
         index, phase, dtype, d, n, rows, q.data_ptr(), q_stride, table.data_ptr(), t_stride, target.data_ptr(),
         0 if weight is None else weight.data_ptr(), scale, 1 if normalize else 0, 0 if loss is None else loss.data_ptr(),
@@ -181,8 +182,9 @@ def _xent(what, phase, q, table, target, scale, normalize, weight=None, loss=Non
     return q, table, target
 
 
-def _floats(n, like):
-    return torch.empty(n, dtype=torch.float32, device=like.device)
+# (tensors come from Tensor.new_empty with sizes as arguments: 1.2 us of host time each, against 1.8 us of torch.empty(shape, device=))
+def _floats(like, *shape):
+    return like.new_empty(*shape, dtype=torch.float32)
 
 
 def softmax_xent_loss(q, table, target, scale=1.0, normalize=False):
@@ -191,7 +193,7 @@ def softmax_xent_loss(q, table, target, scale=1.0, normalize=False):
     ``normalize``: rows count as t / |t| (what the encoder does with the rows it reads; a zero row stays zero), so that unit queries
     score by cosine.  target < 0 ignores a query (loss 0; its lse is still given); target >= rows gives loss NaN."""
     _on_gpu("softmax_xent_loss", q)
-    loss, lse = _floats(q.shape[0], q), _floats(q.shape[0], q)
+    loss, lse = _floats(q, q.shape[0]), _floats(q, q.shape[0])
     _xent("softmax_xent_loss", XENT_LOSS, q, table, target, scale, normalize, loss=loss, lse=lse)
     return loss, lse
 
@@ -202,11 +204,11 @@ def softmax_xent_grads(q, table, target, weight=None, scale=1.0, normalize=False
     dq and dtable have the type of q.  ``grad_table`` (float32, the table's shape): dtable is ADDED there instead, and returned."""
     what = "softmax_xent_grads"
     _on_gpu(what, q, table)
-    loss, lse = _floats(q.shape[0], q), _floats(q.shape[0], q)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    loss, lse = _floats(q, q.shape[0]), _floats(q, q.shape[0])
+    dq = q.new_empty(*q.shape)
     accumulate = grad_table is not None
     if not accumulate:
-        grad_table = torch.empty(table.shape, dtype=table.dtype, device=table.device)
+        grad_table = table.new_empty(*table.shape)
     else:
         _on_gpu(what, q, grad_table)
         d = table.shape[-1]
@@ -222,10 +224,10 @@ class _SoftmaxXent(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, table, target, scale, normalize):
         _on_gpu("softmax_xent", q, table)
-        loss, stat = _floats(q.shape[0], q), _floats((q.shape[0], 2), q)
+        loss, stat = _floats(q, q.shape[0]), _floats(q, q.shape[0], 2)
         dq, phase = None, XENT_LOSS
         if ctx.needs_input_grad[0]:
-            dq, phase = _floats(q.shape, q), XENT_LOSS | XENT_DQ      # of each query's own loss, scaled in backward
+            dq, phase = _floats(q, *q.shape), XENT_LOSS | XENT_DQ      # of each query's own loss, scaled in backward
         q, table, target = _xent("softmax_xent", phase, q, table, target, scale, normalize, loss=loss, stat=stat, dq=dq)
         ctx.save_for_backward(q, table, target, stat, dq)
         ctx.scale, ctx.normalize = scale, normalize
@@ -240,7 +242,7 @@ class _SoftmaxXent(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             gq = (dq * grad.unsqueeze(1)).to(q.dtype)
         if ctx.needs_input_grad[1]:
-            gt = torch.empty(table.shape, dtype=table.dtype, device=table.device)
+            gt = table.new_empty(*table.shape)
             _xent("softmax_xent", XENT_DTABLE, q, table, target, ctx.scale, ctx.normalize, weight=grad, stat=stat, dtable=gt)
         return gq, gt, None, None, None
 
@@ -260,20 +262,26 @@ def softmax_xent(q, table, target, scale=1.0, normalize=False, reduction="mean")
 
 # -- gradient norm and clipping ------------------------------------------------------------------------------------------------
 
+@functools.lru_cache(maxsize=256)
+def _tensors(n):
+    return struct.Struct("@" + n * _TENSOR.format[1:])
+
+
 def _clip(what, grads, max_norm):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if not grads:
         raise ValueError("%s: no tensors" % what)
     index = _on_gpu(what, *grads)
-    parts = []
+    fields = []
     for g in grads:
         if not g.is_contiguous():
             raise ValueError("%s: tensors are contiguous (got shape %s, strides %s)" % (what, tuple(g.shape), g.stride()))
-        parts.append(_TENSOR.pack(g.data_ptr(), g.numel(), _dtype(what, g), 0))
-    n, arr, lib = len(parts), b"".join(parts), library()
+        fields += (g.data_ptr(), g.numel(), _DTYPES.get(g.dtype, -1), 0)
+    if -1 in fields[2::4]:
+        _dtype(what, grads[fields[2::4].index(-1)])      # names it
+    n, arr, lib = len(grads), _tensors(len(grads)).pack(*fields), library()
     need = _check(lib.gqe_clip_grads_workspace(arr, n))
-    space = torch.empty(need, dtype=torch.uint8, device=grads[0].device)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    space, norm = grads[0].new_empty(need, dtype=torch.uint8), grads[0].new_empty((), dtype=torch.float32)
     _check(lib.gqe_clip_grads(index, arr, n, max_norm, norm.data_ptr(), space.data_ptr(), need, _stream(index)))
     return norm
 
@@ -321,8 +329,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     dtype = _dtype(what, x)
     w, b = _ln_vector(what, "weight", weight, index, d), _ln_vector(what, "bias", bias, index, d)
     x, stride = _rows(x)
-    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    mean, rstd = _floats(n, x), _floats(n, x)
+    y, mean, rstd = x.new_empty(n, d), _floats(x, n), _floats(x, n)
     _check(library().gqe_layer_norm_forward(_NORM.pack(index, dtype, d, 0, n, x.data_ptr(), stride, w, b, eps, 0, y.data_ptr(), d, mean.data_ptr(),
                                                        rstd.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, _stream(index))))
     return y, mean, rstd
@@ -345,16 +352,16 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, grad_weight=None, grad_b
     x, x_stride = _rows(x)
     dy, dy_stride = _rows(dy)
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    dx = x.new_empty(n, d)
     accumulate = grad_weight is not None
     if accumulate != (grad_bias is not None):
         raise ValueError("%s: grad_weight and grad_bias come together" % what)
     if accumulate:
         _ln_vector(what, "grad_weight", grad_weight, index, d)
         _ln_vector(what, "grad_bias", grad_bias, index, d)
-    dweight, dbias = (grad_weight, grad_bias) if accumulate else (_floats(d, x), _floats(d, x))
+    dweight, dbias = (grad_weight, grad_bias) if accumulate else (_floats(x, d), _floats(x, d))
     need = _ln_space(dtype, d, n)
-    space = torch.empty(need, dtype=torch.uint8, device=x.device)
+    space = x.new_empty(need, dtype=torch.uint8)
     _check(library().gqe_layer_norm_backward(_NORM.pack(index, dtype, d, 1 if accumulate else 0, n, x.data_ptr(), x_stride, w, 0, 0.0, 0, 0, 0, mean.data_ptr(),
                                                         rstd.data_ptr(), dy.data_ptr(), dy_stride, dx.data_ptr(), d, dweight.data_ptr(),
                                                         dbias.data_ptr(), space.data_ptr(), need, _stream(index))))
