@@ -504,24 +504,18 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
     }
   };
 
-  // stationary rows -> operand registers, through LDS.  Everything that can be is asked for at once, for small problems are a chain of
-  // latencies: the first streamed tiles (DMA: the first, into the one place that the stationary rows do not pass through), all of the
-  // stationary rows (DMA: two tiles at a time), and what belongs to them.
+  // stationary rows -> operand registers.  Everything that can be is asked for at once, the first two streamed tiles too: small problems are
+  // a chain of latencies.
   XentFrag yf[PL][KS];
   float cy = 1.f, ry = 0.f;
   int tgt = -1;
   if (!IS_DT && y_ok) tgt = p.target[y];
-  constexpr int FIRST = DMA && OUT ? L::TILES - 1 : 0;       // the first streamed tile's place
-  if (DMA) {
-    if (y_ok) {
-      const float2 f = p.y_fac[y];
-      cy = f.x;
-      ry = f.y;
-    }
-    if (OUT && tile0 < tile1) load(tile0, FIRST, 0);
-  }
   Feed second;
-  if (!DMA) {
+  if (DMA) {
+#pragma unroll
+    for (int i = 0; i < L::DIST; ++i)
+      if (tile0 + i < tile1) load(tile0 + i, i, i);
+  } else {
     if (tile0 < tile1) load_rows(feed, tile0);
     if (tile0 + 1 < tile1) load_rows(second, tile0 + 1);
   }
@@ -531,17 +525,20 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
 #pragma unroll
       for (int q = 0; q < PL; ++q) *(uint4*)yf[q][ks].u = *(const uint4*)(tile + rs.at(ks >> 2, 32 * (ks & 3)) + q * L::PLANE);
   };
-  if (DMA) {                                     // two tiles at a time
-    const XentDma<BF16, DK> dy = {p.y_image, p.y_stride ? 64 * p.y_stride : (int64_t)L::TILE, 2 * p.y_stride, p.ny};
+  if (DMA) {                                     // straight out of memory: every 128 bytes are used, by four loads in a row
+    if (active) {
+      if (BF16 && p.y_stride) {                  // (a row behind the last one: the last one again, it is not written)
+        const char* from = p.y_image + 2 * (int64_t)(y_ok ? y : p.ny - 1) * p.y_stride + 16 * h;
 #pragma unroll
-    for (int w = 0; w < 4; w += 2) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (yblk * XENT_BM + 32 * (w + i) < p.ny) dy.load(yblk * (XENT_BM / 32) + w + i, lds.tile + i * L::TILE, wave, lane);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (wave >> 1 == w >> 1) take(lds.tile + (wave & 1) * L::TILE);
-      __syncthreads();
+        for (int ks = 0; ks < KS; ++ks) *(uint4*)yf[0][ks].u = *(const uint4*)(from + 32 * ks);
+      } else {
+        take(p.y_image + (int64_t)(y0 / 32) * L::TILE);
+      }
+    }
+    if (y_ok) {
+      const float2 f = p.y_fac[y];
+      cy = f.x;
+      ry = f.y;
     }
     if (IS_DT && h == 0) lds.rn[32 * wave + n] = ry;
   } else {                                       // 32 rows (a wave's) at a time: whole rows are read, and converted once
@@ -648,10 +645,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
 
   if (tile0 < tile1) {
     if (DMA) {
-#pragma unroll
-      for (int i = OUT ? 1 : 0; i < L::DIST; ++i)
-        if (tile0 + i < tile1) load(tile0 + i, (FIRST + i) % L::TILES, i);
-      if (!OUT) arrived();
+      arrived();
     } else {
       feed.st.store(lds.tile, wr);
       factors(feed, tile0, 0);
@@ -661,21 +655,17 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         factors(second, tile0 + 1, 1);
       }
     }
-    if (!DMA || !OUT) __syncthreads();           // (else: the first tile came with the stationary rows)
+    __syncthreads();
     if (active) {
-      product(FIRST, [](int) {});
+      product(0, [](int) {});
 #pragma unroll
       for (int q = 0; q < 4; ++q) exponents(q, 0);
     }
     if (!OUT && !DMA) __syncthreads();           // two tiles: the first one's place is taken next
-    if (DMA && OUT) {
-      arrived();
-      __syncthreads();
-    }
   }
   int mark = 0x7fffffff;                         // DT: target and sign of the next tile's row n
   if (IS_DT && tile0 < tile1) mark = __float_as_int(lds.rec[0].v[3][n]);
-  int tb = FIRST, ab = 0;                        // places of tile t: tile modulo TILES, its rows' part modulo RECS
+  int tb = 0, ab = 0;                            // places of tile t: tile modulo TILES, its rows' part modulo RECS
   for (int t = tile0; t < tile1; ++t) {
     const int tb1 = tb + 1 == L::TILES ? 0 : tb + 1, tb2 = tb1 + 1 == L::TILES ? 0 : tb1 + 1;
     const int ab1 = ab + 1 == L::RECS ? 0 : ab + 1, ab2 = ab1 + 1 == L::RECS ? 0 : ab1 + 1;
