@@ -845,20 +845,22 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
             yf[q][ks].u[i] = sw[0];
             yf[q][ks].u[2 + i] = sw[1];
           }
-      const auto t_of = [&](int ks, int j) {      // element j of the exchanged operands, unit row
-        if (BF16) return (j & 1 ? bf16_hi(yf[0][ks].u[j >> 1]) : bf16_lo(yf[0][ks].u[j >> 1])) * cy;
-        return ((float)yf[0][ks].h[j] + (float)yf[PL - 1][ks].h[j]) * cy;
+      // element j of the exchanged operands; t = cy times it (float32: the sum of its two halves, each a mixed-precision multiply-add)
+      const auto with = [&](int ks, int j, float x, float y) {
+        if (BF16) return fmaf(j & 1 ? bf16_hi(yf[0][ks].u[j >> 1]) : bf16_lo(yf[0][ks].u[j >> 1]), x, y);
+        return fmaf((float)yf[PL - 1][ks].h[j], x, fmaf((float)yf[0][ks].h[j], x, y));
       };
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) along = fmaf(t_of(ks, j), o[ks >> 1][8 * (ks & 1) + j], along);
+        for (int j = 0; j < 8; ++j) along = with(ks, j, o[ks >> 1][8 * (ks & 1) + j], along);
       along += __shfl_xor(along, 32);
+      const float back = -along * cy * cy;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float v = fmaf(-along, t_of(ks, j), o[ks >> 1][8 * (ks & 1) + j]);
+          const float v = with(ks, j, back, o[ks >> 1][8 * (ks & 1) + j]);
           o[ks >> 1][8 * (ks & 1) + j] = v * half * f * rn;
         }
     } else {
