@@ -217,6 +217,42 @@ struct XentLds {
   float rn[XENT_BM];         // DT: 1 / length of the stationary rows, for the end
 };
 
+// Eight elements of a row, as they are: 16 bytes at a time wherever rows begin (the memory takes any alignment), element by element where
+// d cuts them.  Zeros outside.
+template <bool BF16>
+__device__ __forceinline__ void xent_load8(const XentRows& r, int row, int col, uint32_t* raw) {
+#pragma unroll
+  for (int i = 0; i < (BF16 ? 4 : 8); ++i) raw[i] = 0;
+  if (row >= r.n || col >= r.d) return;
+  const int64_t at = (int64_t)row * r.stride + col;
+  if (BF16) {
+    const uint16_t* q = (const uint16_t*)r.p + at;
+    if (col + 8 <= r.d) {
+      const XentU4 u = *(const XentU4*)q;
+      raw[0] = u.v[0]; raw[1] = u.v[1]; raw[2] = u.v[2]; raw[3] = u.v[3];
+    } else {
+      uint32_t e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = col + i < r.d ? q[i] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = e[2 * i] | e[2 * i + 1] << 16;
+    }
+  } else {
+    const float* q = (const float*)r.p + at;
+    if (col + 8 <= r.d) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const XentF4 u = *(const XentF4*)(q + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) raw[i + k] = __float_as_uint(u.v[k]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) raw[i] = col + i < r.d ? __float_as_uint(q[i]) : 0;
+    }
+  }
+}
+
 // One thread's share of 32 rows between their global loads and their LDS stores: 8 threads per row, DK / 8 elements each.
 template <bool BF16, int DK, bool UNIT>
 struct XentStage {
@@ -224,43 +260,9 @@ struct XentStage {
   static constexpr int NCH = DK / 64;          // pieces of 8 elements: piece c of thread t holds columns 64 c + 8 t ..
   uint32_t raw[NCH][BF16 ? 4 : 8];
 
-  // Pieces of 16 bytes wherever rows begin (the memory takes any alignment); a row's last piece element by element where d cuts it.
   __device__ __forceinline__ void load(const XentRows& r, int row, int t8) {
-    const bool ok = row < r.n;
-    const int64_t off = (int64_t)row * r.stride;
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-      const int col = 64 * c + 8 * t8;
-#pragma unroll
-      for (int i = 0; i < (BF16 ? 4 : 8); ++i) raw[c][i] = 0;
-      if (!ok || col >= r.d) continue;
-      if (BF16) {
-        const uint16_t* q = (const uint16_t*)r.p + off + col;
-        if (col + 8 <= r.d) {
-          const XentU4 u = *(const XentU4*)q;
-          raw[c][0] = u.v[0]; raw[c][1] = u.v[1]; raw[c][2] = u.v[2]; raw[c][3] = u.v[3];
-        } else {
-          uint32_t e[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = col + i < r.d ? q[i] : 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) raw[c][i] = e[2 * i] | e[2 * i + 1] << 16;
-        }
-      } else {
-        const float* q = (const float*)r.p + off + col;
-        if (col + 8 <= r.d) {
-#pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            const XentF4 u = *(const XentF4*)(q + i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) raw[c][i + k] = __float_as_uint(u.v[k]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) raw[c][i] = col + i < r.d ? __float_as_uint(q[i]) : 0;
-        }
-      }
-    }
+    for (int c = 0; c < NCH; ++c) xent_load8<BF16>(r, row, 64 * c + 8 * t8, raw[c]);
   }
 
   // Operands into the tile (w: this thread's place), in STEPS pieces of work that a caller may put between matrix instructions:
@@ -447,7 +449,6 @@ template <bool BF16, int DK, int MODE, bool UNIT, bool DMA>
 __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPass p) {
   typedef XentLds<BF16, DK, MODE, DMA> L;
   typedef XentStage<BF16, DK, UNIT && MODE != XENT_MODE_DT> Stage;
-  typedef XentStage<BF16, DK, UNIT && MODE == XENT_MODE_DT> StageY;
   typedef XentTile<DK> Tile;
   extern __shared__ __align__(16) char smem[];
   L& lds = *(L*)smem;
@@ -541,22 +542,57 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
       ry = f.y;
     }
     if (IS_DT && h == 0) lds.rn[32 * wave + n] = ry;
-  } else {                                       // 32 rows (a wave's) at a time: whole rows are read, and converted once
-    StageY st[4];
+  } else if (active) {
+    // Out of the rows themselves, each half of a wave its half of every 16 columns, and converted where they lie: no LDS, no barriers.
+    // (Through LDS, whole rows at a time: 2 to 3 us a workgroup longer, four barriers.)
+    uint32_t raw[KS][BF16 ? 4 : 8];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) st[w].load(yr, yblk * XENT_BM + 32 * w + srow, t8);
+    for (int ks = 0; ks < KS; ++ks) xent_load8<BF16>(yr, y, 16 * ks + 8 * h, raw[ks]);
+    constexpr bool LENGTH = UNIT && IS_DT;
+    float f = 1.f;
+    int k = 0;
+    if (!BF16 || LENGTH) {
+      float mx = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (yblk * XENT_BM + 32 * w >= p.ny) break;
-      st[w].store(lds.tile + (w & 1) * L::TILE, wr);
-      if (t8 == 0) { lds.rec[w & 1].v[0][srow] = st[w].cs; lds.rn[32 * w + srow] = st[w].rn; }
-      __syncthreads();
-      if (wave == w) {
-        take(lds.tile + (w & 1) * L::TILE);
-        cy = lds.rec[w & 1].v[0][n];
-      }
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
+          if (BF16) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(raw[ks][i])), fabsf(bf16_hi(raw[ks][i]))));
+          else mx = fmaxf(mx, fabsf(__uint_as_float(raw[ks][i])));
+        }
+      k = xent_row_scale(fmaxf(mx, __shfl_xor(mx, 32)));
+      f = xent_pow2(k);
     }
-    __syncthreads();
+    ry = 1.f;
+    if (LENGTH) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
+          if (BF16) {
+            const float a = bf16_lo(raw[ks][i]) * f, b = bf16_hi(raw[ks][i]) * f;
+            sum[i & 3] = fmaf(b, b, fmaf(a, a, sum[i & 3]));
+          } else {
+            const float a = __uint_as_float(raw[ks][i]) * f;
+            raw[ks][i] = __float_as_uint(a);
+            sum[i & 3] = fmaf(a, a, sum[i & 3]);
+          }
+        }
+      const float half = (sum[0] + sum[1]) + (sum[2] + sum[3]), g = xent_rsqrt(half + __shfl_xor(half, 32));
+      ry = g * f;
+      k = 14;
+      f = g * 16384.f;
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (BF16) yf[0][ks].u[i] = raw[ks][i];
+        else xent_split(__uint_as_float(raw[ks][2 * i]) * f, __uint_as_float(raw[ks][2 * i + 1]) * f, yf[0][ks].u[i], yf[PL - 1][ks].u[i]);
+      }
+    cy = BF16 ? ry : xent_pow2(-k);
+    if (IS_DT && h == 0) lds.rn[32 * wave + n] = ry;
   }
   if (!IS_DT) cy *= p.scale2;
 
