@@ -140,6 +140,7 @@ struct XentRows {
   const void* p;
   int64_t stride;
   int32_t n, d;
+  __device__ __forceinline__ const char* row(int i, int size) const { return (const char*)p + (i < n ? i : n - 1) * stride * size; }
 };
 struct __attribute__((packed, aligned(2))) XentU4 {
   uint32_t v[4];
@@ -217,38 +218,60 @@ struct XentLds {
   float rn[XENT_BM];         // DT: 1 / length of the stationary rows, for the end
 };
 
-// Eight elements of a row, as they are: 16 bytes at a time wherever rows begin (the memory takes any alignment), element by element where
-// d cuts them.  Zeros outside.
-template <bool BF16>
-__device__ __forceinline__ void xent_load8(const XentRows& r, int row, int col, uint32_t* raw) {
+// Eight elements of a row, as they are: 16 bytes at a time wherever rows begin (the memory takes any alignment).  Rows behind the last one
+// are the last one (their exponents are -inf, their results are not written).  CUT: d may cut the piece; its 16 bytes are then the row's
+// last ones, and xent_cut8 brings them, once they are there, to their places, with zeros behind column d: no branches, for those would
+// keep vector work out of the shadow of matrix instructions (element by element d = 211 cost a third of the whole pass, and code).
+template <bool BF16, bool CUT>
+__device__ __forceinline__ void xent_load8(const char* row, int d, int col, uint32_t* raw) {
+  constexpr int SIZE = BF16 ? 2 : 4, N = BF16 ? 8 : 4;
+  if (CUT && d < N) {                            // (the same for all: a row of less than 16 bytes)
 #pragma unroll
-  for (int i = 0; i < (BF16 ? 4 : 8); ++i) raw[i] = 0;
-  if (row >= r.n || col >= r.d) return;
-  const int64_t at = (int64_t)row * r.stride + col;
-  if (BF16) {
-    const uint16_t* q = (const uint16_t*)r.p + at;
-    if (col + 8 <= r.d) {
-      const XentU4 u = *(const XentU4*)q;
-      raw[0] = u.v[0]; raw[1] = u.v[1]; raw[2] = u.v[2]; raw[3] = u.v[3];
+    for (int i = 0; i < (BF16 ? 4 : 8); ++i) raw[i] = 0;
+    if (col) return;
+    if (BF16) {
+      const uint16_t* q = (const uint16_t*)row;
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (i < d) raw[i >> 1] |= (uint32_t)q[i] << (16 * (i & 1));
     } else {
-      uint32_t e[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = col + i < r.d ? q[i] : 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) raw[i] = e[2 * i] | e[2 * i + 1] << 16;
+      for (int i = 0; i < 3; ++i)
+        if (i < d) raw[i] = ((const uint32_t*)row)[i];
     }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i += N) {
+    const int at = CUT ? min(col + i, d - N) : col + i;
+    const XentU4 u = *(const XentU4*)(row + SIZE * at);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) raw[i + k] = u.v[k];
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void xent_cut8(int d, int col, uint32_t* raw) {
+  constexpr int N = BF16 ? 8 : 4;
+  if (d < N) return;
+  if (BF16) {
+    const int left = d - col, shift = 16 * (8 - left);
+    const uint64_t lo = raw[0] | (uint64_t)raw[1] << 32, hi = raw[2] | (uint64_t)raw[3] << 32;
+    const uint64_t a = shift < 64 ? lo >> (shift & 63) | hi << (64 - shift & 63) : hi >> (shift & 63), b = shift < 64 ? hi >> (shift & 63) : 0;
+    const bool whole = left >= 8, none = left <= 0;
+    raw[0] = whole ? raw[0] : none ? 0 : (uint32_t)a;
+    raw[1] = whole ? raw[1] : none ? 0 : (uint32_t)(a >> 32);
+    raw[2] = whole ? raw[2] : none ? 0 : (uint32_t)b;
+    raw[3] = whole ? raw[3] : none ? 0 : (uint32_t)(b >> 32);
   } else {
-    const float* q = (const float*)r.p + at;
-    if (col + 8 <= r.d) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const XentF4 u = *(const XentF4*)(q + i);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) raw[i + k] = __float_as_uint(u.v[k]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) raw[i] = col + i < r.d ? __float_as_uint(q[i]) : 0;
+    for (int i = 0; i < 8; i += 4) {
+      const int left = d - col - i;
+      const float a = __uint_as_float(raw[i]), b = __uint_as_float(raw[i + 1]), e = __uint_as_float(raw[i + 2]), f = __uint_as_float(raw[i + 3]);
+      const auto pick = [](bool yes, float x, float y) { return yes ? x : y; };
+      raw[i] = __float_as_uint(pick(left >= 4, a, pick(left == 3, b, pick(left == 2, e, pick(left == 1, f, 0.f)))));
+      raw[i + 1] = __float_as_uint(pick(left >= 4, b, pick(left == 3, e, pick(left == 2, f, 0.f))));
+      raw[i + 2] = __float_as_uint(pick(left >= 4, e, pick(left == 3, f, 0.f)));
+      raw[i + 3] = __float_as_uint(pick(left >= 4, f, 0.f));
     }
   }
 }
@@ -260,9 +283,11 @@ struct XentStage {
   static constexpr int NCH = DK / 64;          // pieces of 8 elements: piece c of thread t holds columns 64 c + 8 t ..
   uint32_t raw[NCH][BF16 ? 4 : 8];
 
-  __device__ __forceinline__ void load(const XentRows& r, int row, int t8) {
+  __device__ __forceinline__ void load(const XentRows& r, int row, int t8) {      // (d is more than DK - 64)
+    const char* from = r.row(row, BF16 ? 2 : 4);
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) xent_load8<BF16>(r, row, 64 * c + 8 * t8, raw[c]);
+    for (int c = 0; c < NCH - 1; ++c) xent_load8<BF16, false>(from, r.d, 64 * c + 8 * t8, raw[c]);
+    xent_load8<BF16, true>(from, r.d, 64 * (NCH - 1) + 8 * t8, raw[NCH - 1]);
   }
 
   // Operands into the tile (w: this thread's place), in STEPS pieces of work that a caller may put between matrix instructions:
@@ -273,8 +298,9 @@ struct XentStage {
   int k;
   uint32_t hi[4], lo[4];
 
-  __device__ __forceinline__ void step(int j, char* tile, const XentTile<DK>& w) {
+  __device__ __forceinline__ void step(int j, char* tile, const XentTile<DK>& w, int d, int t8) {
     if (j == 0) {
+      xent_cut8<BF16>(d, 64 * (NCH - 1) + 8 * t8, raw[NCH - 1]);
       k = 0;
       cs = rn = 1.f;
       sum = 0.f;
@@ -334,9 +360,9 @@ struct XentStage {
     }
     if (!BF16 && j == STEPS - 1) cs = xent_pow2(-k);
   }
-  __device__ __forceinline__ void store(char* tile, const XentTile<DK>& w) {
+  __device__ __forceinline__ void store(char* tile, const XentTile<DK>& w, int d, int t8) {
 #pragma unroll
-    for (int j = 0; j < STEPS; ++j) step(j, tile, w);
+    for (int j = 0; j < STEPS; ++j) step(j, tile, w, d, t8);
   }
 };
 
@@ -355,7 +381,7 @@ __device__ __forceinline__ void xent_prep(const XentPrep& p, int which, int tile
   const int row = threadIdx.x >> 3, t8 = threadIdx.x & 7;
   XentStage<BF16, DK, UNIT> st;
   st.load(p.r[which], tile * XENT_TR + row, t8);
-  st.store(turn, XentTile<DK>{xent_full(row, t8), xent_half(row, t8)});
+  st.store(turn, XentTile<DK>{xent_full(row, t8), xent_half(row, t8)}, p.r[which].d, t8);
   if (t8 == 0) {
     const bool ok = tile * XENT_TR + row < p.r[which].n;
     if (ok) p.fac[which][tile * XENT_TR + row] = make_float2(st.cs, st.rn);
@@ -546,8 +572,13 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
     // Out of the rows themselves, each half of a wave its half of every 16 columns, and converted where they lie: no LDS, no barriers.
     // (Through LDS, whole rows at a time: 2 to 3 us a workgroup longer, four barriers.)
     uint32_t raw[KS][BF16 ? 4 : 8];
+    const char* from = yr.row(y, BF16 ? 2 : 4);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) xent_load8<BF16>(yr, y, 16 * ks + 8 * h, raw[ks]);
+    for (int ks = 0; ks < KS - 4; ++ks) xent_load8<BF16, false>(from, p.d, 16 * ks + 8 * h, raw[ks]);
+#pragma unroll
+    for (int ks = KS - 4; ks < KS; ++ks) xent_load8<BF16, true>(from, p.d, 16 * ks + 8 * h, raw[ks]);
+#pragma unroll
+    for (int ks = KS - 4; ks < KS; ++ks) xent_cut8<BF16>(p.d, 16 * ks + 8 * h, raw[ks]);
     constexpr bool LENGTH = UNIT && IS_DT;
     float f = 1.f;
     int k = 0;
@@ -683,11 +714,11 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
     if (DMA) {
       arrived();
     } else {
-      feed.st.store(lds.tile, wr);
+      feed.st.store(lds.tile, wr, p.d, t8);
       factors(feed, tile0, 0);
       if (tile0 + 2 < tile1) load_rows(feed, tile0 + 2);
       if (tile0 + 1 < tile1) {
-        second.st.store(lds.tile + L::TILE, wr);
+        second.st.store(lds.tile + L::TILE, wr, p.d, t8);
         factors(second, tile0 + 1, 1);
       }
     }
@@ -830,7 +861,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
             o[i] = xent_mfma<BF16>(oa[j % (AH + 1)], pf[PL - 1][sk], o[i]);
             o[i] = xent_mfma<BF16>(ol[j % (AH + 1)], pf[0][sk], o[i]);
           }
-          if (!DMA) feed.st.step(j, lds.tile + tb2 * L::TILE, wr);
+          if (!DMA) feed.st.step(j, lds.tile + tb2 * L::TILE, wr, p.d, t8);
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (q * NS / 4 == j) exponents(q, ab1);
@@ -839,7 +870,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         }
       }
     }
-    if (!DMA && (!OUT || !active)) feed.st.store(lds.tile + tb2 * L::TILE, wr);
+    if (!DMA && (!OUT || !active)) feed.st.store(lds.tile + tb2 * L::TILE, wr, p.d, t8);
     if (!OUT && active) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) exponents(q, ab1);
@@ -918,12 +949,12 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         *(float4*)(turn + n * L::OUT_ROW + 32 * i + 8 * q + 4 * h) =
             make_float4(o[2 * c + i][4 * q], o[2 * c + i][4 * q + 1], o[2 * c + i][4 * q + 2], o[2 * c + i][4 * q + 3]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
+#pragma unroll 2
     for (int k = 0; k < 8; ++k) {
       const int row = 4 * k + trow, col = 64 * c + tcol;
       float4 v = *(const float4*)(turn + row * L::OUT_ROW + tcol);
       if (y0 + row < p.ny && col < p.d) {
-        const bool whole = col + 4 <= p.d;
+        const bool whole = c < DK / 64 - 1 || col + 4 <= p.d;
         if (!last) {                             // (columns behind d are zero)
           *(float4*)(p.part_o + ((int64_t)split * p.ny + y0 + row) * p.pitch + col) = v;
         } else if (BF16) {
