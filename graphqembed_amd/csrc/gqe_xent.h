@@ -949,7 +949,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         *(float4*)(turn + n * L::OUT_ROW + 32 * i + 8 * q + 4 * h) =
             make_float4(o[2 * c + i][4 * q], o[2 * c + i][4 * q + 1], o[2 * c + i][4 * q + 2], o[2 * c + i][4 * q + 3]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 2
+#pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int row = 4 * k + trow, col = 64 * c + tcol;
       float4 v = *(const float4*)(turn + row * L::OUT_ROW + tcol);
