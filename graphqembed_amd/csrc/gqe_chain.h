@@ -4,6 +4,7 @@
 // Backward: da = dq r_1 .. r_k through the length into the anchor's row, (da - a (a . da)) / |w|; the relations are the batch's, so their
 // gradients need one column sum, S = sum_b dq_b a_b, and dr_j = S times the other relations.  Anchors repeat: the first query of a row
 // adds up all of that row's gradients in order (a scan over the batch's rows; no atomics, the same bits every time).
+@FIG@
 #ifndef GQE_CHAIN_H
 #define GQE_CHAIN_H
 

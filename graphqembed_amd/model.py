@@ -15,6 +15,8 @@ arena in HBM and every score / gradient is produced by libgqe.so's HIP kernels
 """
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import torch
 import torch.nn as nn
@@ -312,6 +314,8 @@ class QueryEncoderDecoder(nn.Module):
 
     def _softmax_feed(self, items):
         """One upload for all batches: (anchor rows, candidates = target rows - 1, weight_b = loss weight / queries) of each."""
+        if not items:
+            raise Exception("no batches")
         parts, counts = [], []
         for formula, target, anchors, weight in items:
             target = np.ascontiguousarray(target, dtype=np.int32)
@@ -319,6 +323,8 @@ class QueryEncoderDecoder(nn.Module):
             rows = [self.layout.entries[table_key(m)][1][0] for m in (formula.target_mode, formula.anchor_modes[0])]
             if len(target) != len(anchors):
                 raise Exception("%d target and %d anchor rows" % (len(target), len(anchors)))
+            if len(target) > ops.MAX_CHAIN_QUERIES:
+                raise Exception("%d queries in one batch (at most %d)" % (len(target), ops.MAX_CHAIN_QUERIES))
             for r, hi in ((target, rows[0]), (anchors, rows[1])):
                 if len(r) and (r.min() < 0 or r.max() >= hi):
                     raise Exception("a row outside 0 .. %d" % (hi - 1))
@@ -360,6 +366,8 @@ class QueryEncoderDecoder(nn.Module):
         queries; accumulates d(sum_i w_i loss_i) into the gradient arena, loss_i the mean over the batch's queries, and returns
         losses[len(items) + 1] (their weighted sum last).  ``optimizer.step()`` follows, and any margin_step may join it.  The whole
         target table has a gradient: the optimiser's pass covers all of its rows."""
+        if not math.isfinite(scale):
+            raise Exception("scale %r" % (scale,))
         keys = [self._softmax_keys(item[0]) for item in items]
         eng = self.engine
         feed = self._softmax_feed(items)

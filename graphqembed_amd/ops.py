@@ -27,6 +27,7 @@ from .engine import MAX_DIM, GqeError, GqeLibraryError
 
 F32, BF16 = 0, 1
 XENT_LOSS, XENT_DQ, XENT_DTABLE = 1, 2, 4
+MAX_CHAIN_QUERIES = 65536
 _DTYPES = {torch.float32: F32, torch.bfloat16: BF16}
 _P = C.c_void_p
 

@@ -6,7 +6,8 @@
  * Conventions: as in gqe.h — plain C types, borrowed device pointers, all work enqueued on the caller's hipStream_t, no hidden
  * synchronisation, 0 on success or a negative gqe_status.  The calls need no gqe_ctx and keep no state: every buffer they use is an
  * argument, so calls on different streams (with workspaces of their own) and from different threads are independent, and a call can
- * be captured into a HIP graph (kernels only; the workspace then belongs to that graph).  `device` is the HIP device of the pointers
+ * be captured into a HIP graph (kernels only; the workspace then belongs to that graph, and the first call of a kind, which loads its
+ * kernels, comes before).  `device` is the HIP device of the pointers
  * and the stream; it need not be the current one.  gqe_ops_last_error() is the text of the calling thread's last refusal.
  * Rows are `dim` elements with unit stride; row strides are in elements.  Results do not depend on the order of atomics (there are
  * none): the same call on the same inputs gives the same bits. */
@@ -64,7 +65,7 @@ typedef struct {
   int64_t workspace_bytes;
   void* stream;
 } gqe_xent_args;
-int64_t gqe_softmax_xent_workspace(const gqe_xent_args* args);   /* from phase, dtype, dim, n_queries, n_rows; negative: refused */
+int64_t gqe_softmax_xent_workspace(const gqe_xent_args* args);   /* from phase, dtype, dim, n_queries, n_rows and whether stat is given; negative: refused */
 int gqe_softmax_xent(const gqe_xent_args* args);
 
 /* ---- global gradient norm and clipping --------------------------------------------------------------------------------------

@@ -248,8 +248,9 @@ def test_softmax_training_steps_like_torch(lazy):
         assert (off > 1e-4).double().mean().item() <= 0.02, (k, off.max().item())
 
 
-def test_softmax_loss_is_differentiable():
-    model, formulas = build(32)
+@pytest.mark.parametrize("norm", [False, True])
+def test_softmax_loss_is_differentiable(norm):
+    model, formulas = build(32, query_norm=norm)
     f = formulas[1]
     rng = np.random.RandomState(5)
     n = 30
@@ -345,6 +346,34 @@ def test_train_step_with_clipping_is_margin_step_and_step():
     assert torch.allclose(out[0][0], out[1][0], rtol=1e-5) and torch.allclose(out[0][1], out[1][1], rtol=1e-4)
 
 
+def test_softmax_step_on_empty_and_ignored_batches():
+    """A batch without queries and one whose targets are all the dummy row: loss 0, no gradient."""
+    model, formulas = build(32, query_norm=True)
+    none = np.zeros(0, np.int32)
+    items = [(formulas[0], none, none[None], 1.0), (formulas[1], np.zeros(5, np.int32), np.ones((1, 5), np.int32), 2.0)]
+    losses = model.softmax_step(items, 1.5)
+    assert (losses == 0).all() and all(not g.any() for g in read_grads(model).values())
+    assert model.softmax_losses(formulas[0], none, none[None]).shape == (0,)
+
+
+def test_softmax_step_on_another_stream():
+    """The calls follow torch's current stream."""
+    from graphqembed_amd.model import FusedSGD
+    out = []
+    for side in (False, True):
+        model, formulas = build(32, query_norm=True, seed=4)
+        items = batches(formulas, np.random.RandomState(8))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.Stream() if side else torch.cuda.current_stream()):
+            opt = FusedSGD(model, lr=0.1, max_grad_norm=0.5)
+            losses = [model.softmax_step(items, 1.5).clone()]
+            opt.step()
+            losses.append(model.softmax_step(items, 1.5).clone())
+        torch.cuda.synchronize()
+        out.append(torch.stack(losses).cpu())
+    assert torch.equal(out[0], out[1]) and out[0][1, -1] != out[0][0, -1]
+
+
 def test_softmax_refusals():
     from graphqembed_amd.graph import Formula
     from graphqembed_amd.model import FusedAdam
@@ -357,7 +386,11 @@ def test_softmax_refusals():
                  lambda: model.softmax_losses(formulas[0], one, np.ones((1, 4), np.int32))):
         with pytest.raises(Exception):
             call()
-    assert not model._touched
+    for call in (lambda: model.softmax_step([]), lambda: model.softmax_step([(formulas[0], one, one[None], 1.0)], scale=float("inf")),
+                 lambda: model.softmax_step([(formulas[0], np.ones(65537, np.int32), np.ones((1, 65537), np.int32), 1.0)])):
+        with pytest.raises(Exception):
+            call()
+    assert not model._touched and all(not g.any() for g in read_grads(model).values())
     with pytest.raises(ValueError):
         FusedAdam(model, max_grad_norm=float("nan"))
     other, f = build(16, decoder="transe")
