@@ -6,12 +6,14 @@
 // keeps its columns' sums over the rows its group takes, a workgroup adds its groups and writes one row of partial sums, a second
 // launch adds the workgroups' rows in order (no atomics: the same bits every time).  500000 x 256 float32: forward 250 us (4.1 TB/s; with the
 // next row under way while one is summed, 2048 workgroups: the same), backward 308 us (5.0 TB/s) + 5 us of column sums, where a copy of
-// that size reaches 4.8 TB/s; 512 x 128: 3.5 + 3.7 + 2.8 us, launches.
+// that size reaches 4.8 TB/s; 512 x 128: 3.5 + 3.7 us, launches.
 #ifndef GQE_LAYER_NORM_H
 #define GQE_LAYER_NORM_H
 
 #define LN_MAX_DIM 16384
 #define LN_BLOCKS 1024         // workgroups of the backward launch, = rows of partial sums
+#define LN_FEW 2048            // rows up to which weight's and bias's gradients need no launch of their own (2048 x 128: 6.4 us against 3.9 + 3.0, and
+                               // 4 us less of the host's time; 4609 x 257: 20 us against 9 + 5)
 
 struct LnPass {
   const void *x, *dy;
@@ -20,8 +22,9 @@ struct LnPass {
   const float *weight, *bias;
   float *mean, *rstd;
   float* partial;              // [blocks][2][d]
+  float *dweight, *dbias;      // few rows: written by the backward launch itself
   float eps;
-  int32_t d;
+  int32_t d, row_blocks, accumulate;
 };
 
 // N = 16 bytes of elements at any element's alignment (the memory path takes unaligned vectors), the row's end guarded
@@ -142,9 +145,37 @@ __global__ __launch_bounds__(LN_THREADS(G)) void gqe_layer_norm_fwd_kernel(LnPas
   }
 }
 
+// Few rows: the gradients of weight and bias in the same launch, by workgroups of their own behind the rows' (8 columns of all rows each,
+// a share of the rows a thread, shares added in order).
+template <bool BF16, int THREADS>
+__device__ __forceinline__ void ln_columns(const LnPass& p, int block) {
+  constexpr int SHARES = THREADS / 8;
+  __shared__ float lds[2][SHARES][9];
+  const int j = threadIdx.x & 7, k = threadIdx.x >> 3, col = block * 8 + j;
+  float dw = 0.f, db = 0.f;
+  if (col < p.d) {
+#pragma unroll 16
+    for (int row = k; row < (int)p.n; row += SHARES) {
+      const float x = row_elem<BF16>(p.x, row * p.x_stride + col), dy = row_elem<BF16>(p.dy, row * p.dy_stride + col);
+      dw = fmaf(dy, (x - p.mean[row]) * p.rstd[row], dw);
+      db += dy;
+    }
+  }
+  lds[0][k][j] = dw;
+  lds[1][k][j] = db;
+  __syncthreads();
+  if (k > 1 || col >= p.d) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < SHARES; ++i) s += lds[k][i][j];
+  float* out = k ? p.dbias : p.dweight;
+  if (out) out[col] = p.accumulate ? out[col] + s : s;
+}
+
 template <bool BF16, int EPL, int G>
 __global__ __launch_bounds__(LN_THREADS(G)) void gqe_layer_norm_bwd_kernel(LnPass p) {
   constexpr int N = BF16 ? 8 : 4, C = EPL / N, THREADS = LN_THREADS(G), GROUPS = THREADS / G;
+  if ((int)blockIdx.x >= p.row_blocks) return ln_columns<BF16, THREADS>(p, (int)blockIdx.x - p.row_blocks);
   __shared__ float lds[G > 64 ? G / 64 : 1][2];
   __shared__ float cols[GROUPS > 1 ? THREADS * EPL : 1];
   const int g = threadIdx.x / G, t = threadIdx.x % G;
@@ -160,7 +191,7 @@ __global__ __launch_bounds__(LN_THREADS(G)) void gqe_layer_norm_bwd_kernel(LnPas
       for (int i = 0; i < N; i += 4) ln_load<false, 4>(p.weight, (c * G + t) * N + i, p.d, w[c] + i);
   }
   const float over = 1.f / (float)p.d;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + g; row < p.n; row += (int64_t)gridDim.x * GROUPS) {
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + g; row < p.n; row += (int64_t)p.row_blocks * GROUPS) {
     float x[C][N], dy[C][N];
     const char* xr = (const char*)p.x + row * p.x_stride * (BF16 ? 2 : 4);
     const char* gr = (const char*)p.dy + row * p.dy_stride * (BF16 ? 2 : 4);
@@ -315,6 +346,7 @@ LnPass ln_pass(const gqe_layer_norm_args* a) {
   p.x = a->x; p.dy = a->dy; p.y = a->y; p.dx = a->dx;
   p.x_stride = a->x_stride; p.y_stride = a->y_stride; p.dy_stride = a->dy_stride; p.dx_stride = a->dx_stride;
   p.n = a->n_rows; p.weight = a->weight; p.bias = a->bias; p.mean = a->mean; p.rstd = a->rstd; p.eps = a->eps; p.d = a->dim;
+  p.dweight = a->dweight; p.dbias = a->dbias; p.accumulate = a->accumulate;
   return p;
 }
 
@@ -326,7 +358,7 @@ int64_t gqe_layer_norm_workspace(const gqe_layer_norm_args* a) {
   if (!a) return refuse(GQE_ERR_ARG, "layer_norm: args is NULL");
   if ((a->dtype != GQE_F32 && a->dtype != GQE_BF16) || a->dim < 1 || a->dim > LN_MAX_DIM || a->n_rows < 0)
     return refuse(GQE_ERR_ARG, "layer_norm: dtype %d, dim %d, %lld rows", a->dtype, a->dim, (long long)a->n_rows);
-  return (int64_t)ln_blocks(ln_shape(a->dtype == GQE_BF16, a->dim), a->n_rows) * 2 * a->dim * 4;
+  return a->n_rows <= LN_FEW ? 0 : (int64_t)ln_blocks(ln_shape(a->dtype == GQE_BF16, a->dim), a->n_rows) * 2 * a->dim * 4;
 }
 
 int gqe_layer_norm_forward(const gqe_layer_norm_args* a) {
@@ -347,15 +379,18 @@ int gqe_layer_norm_backward(const gqe_layer_norm_args* a) {
   if (!a->dx && !cols) return GQE_OK;
   const LnShape s = ln_shape(a->dtype == GQE_BF16, a->dim);
   const int blocks = ln_blocks(s, a->n_rows);
-  if (cols && (a->workspace_bytes < gqe_layer_norm_workspace(a) || !a->workspace || !aligned(a->workspace, 16)))
-    return refuse(GQE_ERR_WORKSPACE, "layer_norm backward: needs %lld workspace bytes, 16-byte aligned; got %lld", (long long)gqe_layer_norm_workspace(a),
+  const int64_t need = cols ? gqe_layer_norm_workspace(a) : 0;
+  if (need && (a->workspace_bytes < need || !a->workspace || !aligned(a->workspace, 16)))
+    return refuse(GQE_ERR_WORKSPACE, "layer_norm backward: needs %lld workspace bytes, 16-byte aligned; got %lld", (long long)need,
                   (long long)a->workspace_bytes);
   OnDevice dev(a->device);
   if (dev.status != hipSuccess) return hip_refuse(dev.status, "layer_norm backward");
   LnPass p = ln_pass(a);
-  p.partial = cols ? (float*)a->workspace : nullptr;
-  ln_dispatch(a->dtype == GQE_BF16, s, p, true, blocks, (hipStream_t)a->stream);
-  if (cols) gqe_layer_norm_cols_kernel<<<dim3((2 * a->dim + 7) / 8), dim3(256), 0, (hipStream_t)a->stream>>>(p.partial, blocks, a->dim, a->dweight, a->dbias, a->accumulate);
+  p.row_blocks = a->dx || need ? blocks : 0;
+  p.partial = need ? (float*)a->workspace : nullptr;
+  const int extra = cols && !need ? (a->dim + 7) / 8 : 0;
+  ln_dispatch(a->dtype == GQE_BF16, s, p, true, p.row_blocks + extra, (hipStream_t)a->stream);
+  if (need) gqe_layer_norm_cols_kernel<<<dim3((2 * a->dim + 7) / 8), dim3(256), 0, (hipStream_t)a->stream>>>(p.partial, blocks, a->dim, a->dweight, a->dbias, a->accumulate);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? GQE_OK : hip_refuse(e, "layer_norm backward");
 }

@@ -19,6 +19,8 @@ import ctypes as C
 import functools
 import struct
 from collections import OrderedDict
+from itertools import chain, repeat
+from operator import attrgetter
 
 import torch
 
@@ -30,6 +32,7 @@ XENT_LOSS, XENT_DQ, XENT_DTABLE = 1, 2, 4
 MAX_CHAIN_QUERIES = 65536
 _DTYPES = {torch.float32: F32, torch.bfloat16: BF16}
 _P = C.c_void_p
+_DEVICE_OF, _DTYPE_OF = torch.Tensor.get_device, attrgetter("dtype")
 
 
 class gqe_xent_args(C.Structure):
@@ -272,15 +275,19 @@ def _clip(what, grads, max_norm):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if not grads:
         raise ValueError("%s: no tensors" % what)
-    index = _on_gpu(what, *grads)
-    fields = []
-    for g in grads:
-        if not g.is_contiguous():
+    try:
+        devices = set(map(_DEVICE_OF, grads))
+    except TypeError:
+        devices = ()
+    index = _on_gpu(what, *grads) if len(devices) != 1 or -1 in devices else devices.pop()      # (names what is wrong)
+    for g, contiguous in zip(grads, map(torch.Tensor.is_contiguous, grads)):
+        if not contiguous:
             raise ValueError("%s: tensors are contiguous (got shape %s, strides %s)" % (what, tuple(g.shape), g.stride()))
-        fields += (g.data_ptr(), g.numel(), _DTYPES.get(g.dtype, -1), 0)
-    if -1 in fields[2::4]:
-        _dtype(what, grads[fields[2::4].index(-1)])      # names it
-    n, arr, lib = len(grads), _tensors(len(grads)).pack(*fields), library()
+    codes = [_DTYPES.get(t) for t in map(_DTYPE_OF, grads)]
+    if None in codes:
+        _dtype(what, grads[codes.index(None)])
+    n, lib = len(grads), library()
+    arr = _tensors(n).pack(*chain.from_iterable(zip(map(torch.Tensor.data_ptr, grads), map(torch.Tensor.numel, grads), codes, repeat(0))))
     need = _check(lib.gqe_clip_grads_workspace(arr, n))
     space, norm = grads[0].new_empty(need, dtype=torch.uint8), grads[0].new_empty((), dtype=torch.float32)
     _check(lib.gqe_clip_grads(index, arr, n, max_norm, norm.data_ptr(), space.data_ptr(), need, _stream(index)))
@@ -362,10 +369,10 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, grad_weight=None, grad_b
         _ln_vector(what, "grad_bias", grad_bias, index, d)
     dweight, dbias = (grad_weight, grad_bias) if accumulate else (_floats(x, d), _floats(x, d))
     need = _ln_space(dtype, d, n)
-    space = x.new_empty(need, dtype=torch.uint8)
+    space = x.new_empty(need, dtype=torch.uint8) if need else None
     _check(library().gqe_layer_norm_backward(_NORM.pack(index, dtype, d, 1 if accumulate else 0, n, x.data_ptr(), x_stride, w, 0, 0.0, 0, 0, 0, mean.data_ptr(),
                                                         rstd.data_ptr(), dy.data_ptr(), dy_stride, dx.data_ptr(), d, dweight.data_ptr(),
-                                                        dbias.data_ptr(), space.data_ptr(), need, _stream(index))))
+                                                        dbias.data_ptr(), space.data_ptr() if need else 0, need, _stream(index))))
     return dx, dweight, dbias
 
 

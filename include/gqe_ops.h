@@ -109,7 +109,7 @@ typedef struct {
   int64_t dx_stride;
   float* dweight;
   float* dbias;
-  void* workspace;          /* gqe_layer_norm_workspace bytes (backward with dweight or dbias) */
+  void* workspace;          /* gqe_layer_norm_workspace bytes (backward with dweight or dbias; 0 for few rows) */
   int64_t workspace_bytes;
   void* stream;
 } gqe_layer_norm_args;

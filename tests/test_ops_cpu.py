@@ -110,6 +110,9 @@ def test_layer_norm_refuses_what_one_direction_needs(ops):
     assert lib.gqe_layer_norm_forward(C.byref(a)) == -1 and "y is NULL" in lib.gqe_ops_last_error().decode()
     assert lib.gqe_layer_norm_backward(C.byref(a)) == -1 and "dy is NULL" in lib.gqe_ops_last_error().decode()
     a.dy = a.dweight = 1 << 20
+    assert lib.gqe_layer_norm_workspace(C.byref(a)) == 0                      # few rows: one launch, no workspace
+    a.n_rows = 5000
+    assert lib.gqe_layer_norm_workspace(C.byref(a)) > 0
     assert lib.gqe_layer_norm_backward(C.byref(a)) == -5 and "workspace" in lib.gqe_ops_last_error().decode()
 
 
