@@ -4,14 +4,16 @@
 // threads (a part of a wave, a wave, or a workgroup), EPL elements each in 16-byte pieces, so mean and variance are two passes
 // over registers (no cancellation) and nothing is read twice.  The weight's and bias's gradients are column sums: each thread
 // keeps its columns' sums over the rows its group takes, a workgroup adds its groups and writes one row of partial sums, a second
-// launch adds the workgroups' rows in order (no atomics: the same bits every time).  500000 x 256 float32: forward 250 us (4.1 TB/s; with the
-// next row under way while one is summed, 2048 workgroups: the same), backward 308 us (5.0 TB/s) + 5 us of column sums, where a copy of
+// launch adds the workgroups' rows in order (no atomics: the same bits every time).  500000 x 256 float32: forward 240 us (4.3 TB/s; with the
+// next row under way while one is summed, 2048 workgroups: the same), backward 275 us (5.6 TB/s) + 5 us of column sums, where a copy of
 // that size reaches 4.8 TB/s; 512 x 128: 3.5 + 3.7 us, launches.
 #ifndef GQE_LAYER_NORM_H
 #define GQE_LAYER_NORM_H
 
 #define LN_MAX_DIM 16384
 #define LN_BLOCKS 1024         // workgroups of the backward launch, = rows of partial sums
+#define LN_STREAM (64LL << 20)    // bytes of an output from which it is written past the caches: 154 MB forward 76 -> 60 us, backward 89 -> 69; 512 MB 247 -> 240 and
+                               // 299 -> 275; 55 MB the same (and there whoever reads it next finds it)
 #define LN_FEW 2048            // rows up to which weight's and bias's gradients need no launch of their own (2048 x 128: 6.4 us against 3.9 + 3.0, and
                                // 4 us less of the host's time; 4609 x 257: 20 us against 9 + 5)
 
@@ -24,7 +26,7 @@ struct LnPass {
   float* partial;              // [blocks][2][d]
   float *dweight, *dbias;      // few rows: written by the backward launch itself
   float eps;
-  int32_t d, row_blocks, accumulate;
+  int32_t d, row_blocks, accumulate, stream;
 };
 
 // N = 16 bytes of elements at any element's alignment (the memory path takes unaligned vectors), the row's end guarded
@@ -51,14 +53,18 @@ __device__ __forceinline__ void ln_load(const void* row, int col, int d, float* 
     }
   }
 }
-template <bool BF16, int N>
+// STREAM: past the caches (LnPass::stream)
+typedef uint32_t ln_u4 __attribute__((ext_vector_type(4), aligned(2)));
+template <bool BF16, int N, bool STREAM = false>
 __device__ __forceinline__ void ln_store(void* row, int col, int d, const float* v) {
   if (BF16) {
     uint16_t* p = (uint16_t*)row + col;
     uint32_t u[N / 2];
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) u[i] = xent_pack_bf16(v[2 * i], v[2 * i + 1]);
-    if (col + N <= d) {
+    if (STREAM && col + N <= d) {
+      __builtin_nontemporal_store((ln_u4){u[0], u[1], u[2], u[3]}, (ln_u4*)p);
+    } else if (col + N <= d) {
       __builtin_memcpy(p, u, 2 * N);
     } else {
 #pragma unroll
@@ -67,7 +73,9 @@ __device__ __forceinline__ void ln_store(void* row, int col, int d, const float*
     }
   } else {
     float* p = (float*)row + col;
-    if (col + N <= d) {
+    if (STREAM && col + N <= d) {
+      __builtin_nontemporal_store((ln_u4){__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}, (ln_u4*)p);
+    } else if (col + N <= d) {
       __builtin_memcpy(p, v, 4 * N);
     } else {
 #pragma unroll
@@ -141,7 +149,8 @@ __global__ __launch_bounds__(LN_THREADS(G)) void gqe_layer_norm_fwd_kernel(LnPas
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) x[c][i] = fmaf(x[c][i] * rstd, w[i], b[i]);
-    ln_store<BF16, N>(yr, col, p.d, x[c]);
+    if (p.stream) ln_store<BF16, N, true>(yr, col, p.d, x[c]);
+    else ln_store<BF16, N>(yr, col, p.d, x[c]);
   }
 }
 
@@ -222,7 +231,8 @@ __global__ __launch_bounds__(LN_THREADS(G)) void gqe_layer_norm_bwd_kernel(LnPas
       for (int c = 0; c < C; ++c) {
 #pragma unroll
         for (int i = 0; i < N; ++i) dy[c][i] = rstd * (dy[c][i] - a - x[c][i] * b);
-        ln_store<BF16, N>(out, (c * G + t) * N, p.d, dy[c]);
+        if (p.stream) ln_store<BF16, N, true>(out, (c * G + t) * N, p.d, dy[c]);
+        else ln_store<BF16, N>(out, (c * G + t) * N, p.d, dy[c]);
       }
     }
   }
@@ -346,6 +356,7 @@ LnPass ln_pass(const gqe_layer_norm_args* a) {
   p.x = a->x; p.dy = a->dy; p.y = a->y; p.dx = a->dx;
   p.x_stride = a->x_stride; p.y_stride = a->y_stride; p.dy_stride = a->dy_stride; p.dx_stride = a->dx_stride;
   p.n = a->n_rows; p.weight = a->weight; p.bias = a->bias; p.mean = a->mean; p.rstd = a->rstd; p.eps = a->eps; p.d = a->dim;
+  p.stream = a->n_rows * a->dim * (a->dtype == GQE_BF16 ? 2 : 4) > LN_STREAM;
   p.dweight = a->dweight; p.dbias = a->dbias; p.accumulate = a->accumulate;
   return p;
 }

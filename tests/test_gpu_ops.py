@@ -520,6 +520,25 @@ def test_layer_norm_views_and_autograd():
     assert abs((f(x + h * v) - f(x - h * v)) / (2 * h) - (xa.grad.double() * v.double()).sum().item()) < 0.02
 
 
+@pytest.mark.parametrize("n,d,dtype", [(33000, 513, torch.float32), (17000, 1024, torch.float32), (70001, 481, torch.bfloat16)])
+def test_layer_norm_of_large_outputs(n, d, dtype):
+    """Outputs that are written past the caches: row for row the bits of a small call, the columns' sums by the formula."""
+    from graphqembed_amd import ops
+    x, dy = torch.randn(n, d, device="cuda").to(dtype), torch.randn(n, d, device="cuda").to(dtype)
+    w, b = torch.rand(d, device="cuda") + 0.5, torch.randn(d, device="cuda")
+    y, mean, rstd = ops.layer_norm_forward(x, w, b)
+    dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, w)
+    for i in (0, n // 2, n - 700):
+        part = slice(i, i + 700)
+        y2, mean2, rstd2 = ops.layer_norm_forward(x[part], w, b)
+        dx2, _, _ = ops.layer_norm_backward(dy[part], x[part], mean2, rstd2, w)
+        assert torch.equal(y[part], y2) and torch.equal(dx[part], dx2) and torch.equal(mean[part], mean2) and torch.equal(rstd[part], rstd2)
+    h = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    kn = (2 * (40 + math.log2(n)) + 2 * (n // 1024)) * U                # as above; xhat itself rounds 3 times more
+    assert ((dw.double() - (dy.double() * h).sum(0)).abs() <= (kn + 4 * U) * (dy.double() * h).abs().sum(0)).all()
+    assert ((db.double() - dy.double().sum(0)).abs() <= kn * dy.double().abs().sum(0)).all()
+
+
 def test_layer_norm_edges_and_refusals():
     from graphqembed_amd import ops
     flat = torch.full((4, 50), 3.0, device="cuda")
