@@ -737,7 +737,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
 #pragma unroll
       for (int q = 0; q < 4; ++q) exponents(q, 0);
     }
-    if (!OUT && !DMA) __syncthreads();           // two tiles: the first one's place is taken next
+    if (!OUT) __syncthreads();                   // two places: the first one is taken next, when everyone has read it
   }
   int mark = 0x7fffffff;                         // DT: target and sign of the next tile's row n
   if (IS_DT && tile0 < tile1) mark = __float_as_int(lds.rec[0].v[3][n]);

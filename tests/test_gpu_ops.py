@@ -102,6 +102,21 @@ def test_softmax_xent_grads(B, V, d, normalize, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,V,d", [(333, 75842, 206), (700, 30001, 256), (1500, 9000, 100), (260, 60000, 48)])
+def test_softmax_xent_losses_of_long_streams(B, V, d, dtype):
+    """Losses alone take a tile's place for the next but one: many tiles to a workgroup, call after call the same bits."""
+    from graphqembed_amd import ops
+    for seed in range(6):
+        q, table, target, weight = xent_inputs(B, V, d, dtype, seed=seed)
+        loss, lse = ops.softmax_xent_loss(q, table, target)
+        e = xent_exact(q, table, target, weight, 1.0, False)
+        check_xent((loss, lse, None, None), e, dtype, False, seed)
+        for _ in range(20):
+            again = ops.softmax_xent_loss(q, table, target)
+            assert torch.equal(again[0], loss) and torch.equal(again[1], lse), seed
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_softmax_xent_strided_and_unaligned(dtype):
     """Views: rows 1 .. n of a wider buffer at an odd element offset, 64-bit targets, weights of every sign, a negative scale."""
     from graphqembed_amd import ops
