@@ -221,7 +221,7 @@ struct XentLds {
   static constexpr int TILES = (MODE == XENT_MODE_LSE ? 0 : 1) + DIST;
   static constexpr int RECS = DIST + 1;
   static constexpr int OUT_ROW = 68;                                  // floats of a row of the outputs' turn (64 columns at a time)
-  static constexpr int OUT = MODE == XENT_MODE_LSE ? 0 : 4 * 32 * OUT_ROW * 4;
+  static constexpr int OUT = MODE == XENT_MODE_LSE ? (DMA ? 0 : 4 * PLANES * 4096) : 4 * 32 * OUT_ROW * 4;      // (LSE: the stationary rows' way in)
   char tile[TILES * TILE > OUT ? TILES * TILE : OUT];
   XentRec rec[RECS];
   float rn[XENT_BM];         // DT: 1 / length of the stationary rows, for the end
@@ -307,54 +307,83 @@ struct XentStage {
   int k;
   uint32_t hi[4], lo[4];
 
+  __device__ __forceinline__ void largest(int d, int t8) {
+    xent_cut8<BF16>(d, 64 * (NCH - 1) + 8 * t8, raw[NCH - 1]);
+    k = 0;
+    cs = rn = 1.f;
+    sum = 0.f;
+    if (BF16 && !UNIT) return;
+    float mx = 0.f;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+      for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
+        if (BF16) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(raw[c][i])), fabsf(bf16_hi(raw[c][i]))));
+        else mx = fmaxf(mx, fabsf(__uint_as_float(raw[c][i])));
+      }
+    mx = fmaxf(mx, dpp_get<0xB1, 0xF>(mx));        // the row's 8 threads: swaps in fours, then halves mirrored
+    mx = fmaxf(mx, dpp_get<0x4E, 0xF>(mx));
+    mx = fmaxf(mx, dpp_get<0x141, 0xF>(mx));
+    k = xent_row_scale(mx);
+    f = xent_pow2(k);
+  }
+  __device__ __forceinline__ void squares(int c) {
+#pragma unroll
+    for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
+      if (BF16) {
+        const float a = bf16_lo(raw[c][i]) * f, b = bf16_hi(raw[c][i]) * f;
+        sum = fmaf(a, a, sum);
+        sum = fmaf(b, b, sum);
+      } else {
+        const float a = __uint_as_float(raw[c][i]) * f;
+        raw[c][i] = __float_as_uint(a);
+        sum = fmaf(a, a, sum);
+      }
+    }
+  }
+  __device__ __forceinline__ void length() {
+    sum += dpp_get<0xB1, 0xF>(sum);
+    sum += dpp_get<0x4E, 0xF>(sum);
+    sum += dpp_get<0x141, 0xF>(sum);
+    const float g = xent_rsqrt(sum);
+    rn = g * f;
+    cs = rn;
+    k = 14;
+    f = g * 16384.f;
+  }
+  // all of that at once, and then piece c
+  __device__ __forceinline__ void scale(int d, int t8) {
+    largest(d, t8);
+    if (UNIT) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) squares(c);
+      length();
+    }
+    if (!BF16) cs = xent_pow2(-k);
+  }
+  __device__ __forceinline__ void piece(int c, uint4& a, uint4& b) const {
+    if (BF16) {
+      a = make_uint4(raw[c][0], raw[c][1], raw[c][2], raw[c][3]);
+      return;
+    }
+    uint32_t x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xent_split(__uint_as_float(raw[c][2 * i]) * f, __uint_as_float(raw[c][2 * i + 1]) * f, x[i], y[i]);
+    a = make_uint4(x[0], x[1], x[2], x[3]);
+    b = make_uint4(y[0], y[1], y[2], y[3]);
+  }
+
   __device__ __forceinline__ void step(int j, char* tile, const XentTile<DK>& w, int d, int t8) {
     if (j == 0) {
-      xent_cut8<BF16>(d, 64 * (NCH - 1) + 8 * t8, raw[NCH - 1]);
-      k = 0;
-      cs = rn = 1.f;
-      sum = 0.f;
+      largest(d, t8);
       if (BF16) {
 #pragma unroll
         for (int c = 0; c < NCH; ++c) *(uint4*)(tile + w.at(c, 0)) = make_uint4(raw[c][0], raw[c][1], raw[c][2], raw[c][3]);
       }
-      if (!BF16 || UNIT) {
-        float mx = 0.f;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c)
-#pragma unroll
-          for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
-            if (BF16) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(raw[c][i])), fabsf(bf16_hi(raw[c][i]))));
-            else mx = fmaxf(mx, fabsf(__uint_as_float(raw[c][i])));
-          }
-        mx = fmaxf(mx, dpp_get<0xB1, 0xF>(mx));        // the row's 8 threads: swaps in fours, then halves mirrored
-        mx = fmaxf(mx, dpp_get<0x4E, 0xF>(mx));
-        mx = fmaxf(mx, dpp_get<0x141, 0xF>(mx));
-        k = xent_row_scale(mx);
-        f = xent_pow2(k);
-      }
     } else if (UNIT && j <= NCH) {
-      const int c = j - 1;
-#pragma unroll
-      for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
-        if (BF16) {
-          const float a = bf16_lo(raw[c][i]) * f, b = bf16_hi(raw[c][i]) * f;
-          sum = fmaf(a, a, sum);
-          sum = fmaf(b, b, sum);
-        } else {
-          const float a = __uint_as_float(raw[c][i]) * f;
-          raw[c][i] = __float_as_uint(a);
-          sum = fmaf(a, a, sum);
-        }
-      }
+      squares(j - 1);
     } else if (UNIT && j == NCH + 1) {
-      sum += dpp_get<0xB1, 0xF>(sum);
-      sum += dpp_get<0x4E, 0xF>(sum);
-      sum += dpp_get<0x141, 0xF>(sum);
-      const float g = xent_rsqrt(sum);
-      rn = g * f;
-      cs = rn;
-      k = 14;
-      f = g * 16384.f;
+      length();
     } else if (!BF16 && j >= HEAD) {
 #pragma unroll
       for (int q = (j - HEAD) * PER; q < (j - HEAD + 1) * PER && q < STEPS; ++q) {
@@ -484,6 +513,7 @@ template <bool BF16, int DK, int MODE, bool UNIT, bool DMA>
 __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPass p) {
   typedef XentLds<BF16, DK, MODE, DMA> L;
   typedef XentStage<BF16, DK, UNIT && MODE != XENT_MODE_DT> Stage;
+  typedef XentStage<BF16, DK, UNIT && MODE == XENT_MODE_DT> Own;
   typedef XentTile<DK> Tile;
   extern __shared__ __align__(16) char smem[];
   L& lds = *(L*)smem;
@@ -578,60 +608,39 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
     }
     if (IS_DT && h == 0) lds.rn[32 * wave + n] = ry;
   } else if (active) {
-    // Out of the rows themselves, each half of a wave its half of every 16 columns, and converted where they lie: no LDS, no barriers.
-    // (Through LDS, whole rows at a time: 2 to 3 us a workgroup longer, four barriers.)
-    uint32_t raw[KS][BF16 ? 4 : 8];
-    const char* from = yr.row(y, BF16 ? 2 : 4);
+    // Each wave its own 32 rows, eight threads a row (whole cache lines), four rows a thread; converted, and turned into operands by way of
+    // 4 KB of LDS a plane that no other wave touches: no barriers.  (Read in the operands' own order, 32 bytes of 32 rows at a time,
+    // 128 rows of 1 KB took 6 us instead of 3.)
+    char* mine = lds.tile + wave * PL * 4096;
+    const int r8 = lane >> 3;
+    Own own[4];
 #pragma unroll
-    for (int ks = 0; ks < KS - 4; ++ks) xent_load8<BF16, false>(from, p.d, 16 * ks + 8 * h, raw[ks]);
+    for (int g = 0; g < 4; ++g) own[g].load(yr, y0 + 8 * g + r8, t8);
 #pragma unroll
-    for (int ks = KS - 4; ks < KS; ++ks) xent_load8<BF16, true>(from, p.d, 16 * ks + 8 * h, raw[ks]);
+    for (int g = 0; g < 4; ++g) own[g].scale(p.d, t8);
 #pragma unroll
-    for (int ks = KS - 4; ks < KS; ++ks) xent_cut8<BF16>(p.d, 16 * ks + 8 * h, raw[ks]);
-    constexpr bool LENGTH = UNIT && IS_DT;
-    float f = 1.f;
-    int k = 0;
-    if (!BF16 || LENGTH) {
-      float mx = 0.f;
+    for (int c = 0; c < DK / 64; ++c) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
-          if (BF16) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(raw[ks][i])), fabsf(bf16_hi(raw[ks][i]))));
-          else mx = fmaxf(mx, fabsf(__uint_as_float(raw[ks][i])));
-        }
-      k = xent_row_scale(fmaxf(mx, __shfl_xor(mx, 32)));
-      f = xent_pow2(k);
-    }
-    ry = 1.f;
-    if (LENGTH) {
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
-          if (BF16) {
-            const float a = bf16_lo(raw[ks][i]) * f, b = bf16_hi(raw[ks][i]) * f;
-            sum[i & 3] = fmaf(b, b, fmaf(a, a, sum[i & 3]));
-          } else {
-            const float a = __uint_as_float(raw[ks][i]) * f;
-            raw[ks][i] = __float_as_uint(a);
-            sum[i & 3] = fmaf(a, a, sum[i & 3]);
-          }
-        }
-      const float half = (sum[0] + sum[1]) + (sum[2] + sum[3]), g = xent_rsqrt(half + __shfl_xor(half, 32));
-      ry = g * f;
-      k = 14;
-      f = g * 16384.f;
-    }
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (BF16) yf[0][ks].u[i] = raw[ks][i];
-        else xent_split(__uint_as_float(raw[ks][2 * i]) * f, __uint_as_float(raw[ks][2 * i + 1]) * f, yf[0][ks].u[i], yf[PL - 1][ks].u[i]);
+      for (int g = 0; g < 4; ++g) {
+        uint4 hi, lo = make_uint4(0, 0, 0, 0);
+        own[g].piece(c, hi, lo);
+        char* to = mine + xent_half(8 * g + r8, t8);
+        *(uint4*)to = hi;
+        if (!BF16) *(uint4*)(to + 4096) = lo;
       }
-    cy = BF16 ? ry : xent_pow2(-k);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+        for (int q = 0; q < PL; ++q) *(uint4*)yf[q][4 * c + ks].u = *(const uint4*)(mine + q * 4096 + (rs.half ^ (32 * ks)));
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {                // each row's factors to the lanes that now hold it
+      const float c = __shfl(own[g].cs, 8 * (n & 7)), r = __shfl(own[g].rn, 8 * (n & 7));
+      if (n >> 3 == g) {
+        cy = c;
+        ry = r;
+      }
+    }
     if (IS_DT && h == 0) lds.rn[32 * wave + n] = ry;
   }
   if (!IS_DT) cy *= p.scale2;
@@ -723,6 +732,7 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
     if (DMA) {
       arrived();
     } else {
+      __syncthreads();                           // the stationary rows have passed
       feed.st.store(lds.tile, wr, p.d, t8);
       factors(feed, tile0, 0);
       if (tile0 + 2 < tile1) load_rows(feed, tile0 + 2);
