@@ -29,7 +29,8 @@
 // bfloat16, 4608 x 131071 x 256: 830 + 940 us = 700 TFLOP/s; one wave per SIMD holds 330 registers, so vector work (7 instructions and an
 // exponential a number), the tile's loads (18 %) and the first product's chain (21 %) add up instead of hiding behind other waves;
 // d <= 192, two waves per SIMD, gains 40 %.  64 stationary rows a wave (half the LDS traffic) were no faster at d = 128 and do not fit at
-// 256.  Few queries: memory, at 2.2 TB/s where a table of 352 MB is read twice and written once (6 x 427109 x 206: 162 + 219 us).
+// 256.  Few queries (6 x 427109 x 206: 153 + 199 us): memory, at 2.3 TB/s in the first pass, where three waves of four only convert, and 3.5
+// in the second, where a workgroup is 1 us of starting, 3 of reading, 4 of products for one tile, 3 of the length's gradient and 3 of writing.
 #ifndef GQE_XENT_H
 #define GQE_XENT_H
 
@@ -956,9 +957,17 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         for (int r = 0; r < 16; ++r) o[i][r] *= half * f;
     }
   }
-  // 64 columns at a time through LDS, so that whole pieces of rows are written
+  // 64 columns at a time through LDS, so that whole pieces of rows are written.  Partial sums have rows of whole 16 bytes, zero behind d.
   float* turn = (float*)lds.tile + wave * 32 * L::OUT_ROW;
   const int trow = here >> 4, tcol = 4 * (here & 15);
+  const bool half = BF16 && last;                // bfloat16 results
+  const int size = half ? 2 : 4;
+  const int64_t stride = (last ? p.out_stride : (int64_t)p.pitch) * size;
+  const int width = last ? p.d : p.pitch, rows = p.ny - y0 - trow;       // rows 4 k + trow, while 4 k is less
+  char* to[8];
+  to[0] = (last ? (char*)p.out : (char*)(p.part_o + (int64_t)split * p.ny * p.pitch)) + (y0 + trow) * stride + tcol * size;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) to[k] = to[k - 1] + 4 * stride;
 #pragma unroll
   for (int c = 0; c < DK / 64; ++c) {
 #pragma unroll
@@ -968,37 +977,50 @@ __global__ __launch_bounds__(256, XENT_TWO ? 2 : 1) void gqe_xent_kernel(XentPas
         *(float4*)(turn + n * L::OUT_ROW + 32 * i + 8 * q + 4 * h) =
             make_float4(o[2 * c + i][4 * q], o[2 * c + i][4 * q + 1], o[2 * c + i][4 * q + 2], o[2 * c + i][4 * q + 3]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int left = width - 64 * c - tcol;      // columns from here on
+    const bool some = c < DK / 64 - 1 || left > 0, whole = c < DK / 64 - 1 || left >= 4;
+    const auto write = [&](auto&& one) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int row = 4 * k + trow, col = 64 * c + tcol;
-      float4 v = *(const float4*)(turn + row * L::OUT_ROW + tcol);
-      if (y0 + row < p.ny && col < p.d) {
-        const bool whole = c < DK / 64 - 1 || col + 4 <= p.d;
-        if (!last) {                             // (columns behind d are zero)
-          *(float4*)(p.part_o + ((int64_t)split * p.ny + y0 + row) * p.pitch + col) = v;
-        } else if (BF16) {
-          uint16_t* po = (uint16_t*)p.out + (int64_t)(y0 + row) * p.out_stride + col;
-          const uint32_t a = xent_pack_bf16(v.x, v.y), b = xent_pack_bf16(v.z, v.w);
-          if (whole) {
-            *(XentU2*)po = XentU2{{a, b}};
-          } else {
-            po[0] = (uint16_t)a;
-            if (col + 1 < p.d) po[1] = (uint16_t)(a >> 16);
-            if (col + 2 < p.d) po[2] = (uint16_t)b;
-          }
-        } else {
-          float* po = (float*)p.out + (int64_t)(y0 + row) * p.out_stride + col;
-          if (whole) {
-            if (p.accumulate) { const XentF4 w = *(const XentF4*)po; v.x += w.v[0]; v.y += w.v[1]; v.z += w.v[2]; v.w += w.v[3]; }
-            *(XentF4*)po = XentF4{{v.x, v.y, v.z, v.w}};
-          } else {
-            const float e4[3] = {v.x, v.y, v.z};
-#pragma unroll
-            for (int j = 0; j < 3; ++j)
-              if (col + j < p.d) po[j] = p.accumulate ? po[j] + e4[j] : e4[j];
-          }
-        }
+      for (int k = 0; k < 8; ++k) {
+        const float4 v = *(const float4*)(turn + (4 * k + trow) * L::OUT_ROW + tcol);
+        if (some && 4 * k < rows) one(to[k] + 64 * c * size, v);
       }
+    };
+    if (half) {
+      write([&](char* at, const float4& v) {
+        const uint32_t a = xent_pack_bf16(v.x, v.y), b = xent_pack_bf16(v.z, v.w);
+        if (whole) {
+          *(XentU2*)at = XentU2{{a, b}};
+        } else {
+          uint16_t* po = (uint16_t*)at;
+          po[0] = (uint16_t)a;
+          if (left > 1) po[1] = (uint16_t)(a >> 16);
+          if (left > 2) po[2] = (uint16_t)b;
+        }
+      });
+    } else if (last && p.accumulate) {
+      write([&](char* at, const float4& v) {
+        float* po = (float*)at;
+        if (whole) {
+          const XentF4 w = *(const XentF4*)po;
+          *(XentF4*)po = XentF4{{w.v[0] + v.x, w.v[1] + v.y, w.v[2] + v.z, w.v[3] + v.w}};
+        } else {
+          po[0] += v.x;
+          if (left > 1) po[1] += v.y;
+          if (left > 2) po[2] += v.z;
+        }
+      });
+    } else {
+      write([&](char* at, const float4& v) {
+        if (whole) {
+          *(XentF4*)at = XentF4{{v.x, v.y, v.z, v.w}};
+        } else {
+          float* po = (float*)at;
+          po[0] = v.x;
+          if (left > 1) po[1] = v.y;
+          if (left > 2) po[2] = v.z;
+        }
+      });
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
