@@ -99,17 +99,6 @@ __device__ __forceinline__ double wave_sum_f64(double x) {
   for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
   return x;
 }
-// 2^x and log2 x of a 64-bit number to float32's relative (absolute, below 1) precision: whole powers apart, the rest in float32
-__device__ __forceinline__ float exp2_of(double x) {
-  const double n = floor(fmax(x, -1000.0));
-  return ldexpf(exp2f((float)(x - n)), (int)n);
-}
-__device__ __forceinline__ double log2_of(double x) {
-  int e;
-  const double f = frexp(x, &e);
-  return x > 0.0 ? (double)(e - 1) + (double)log2f((float)(f + f)) : x == 0.0 ? -INFINITY : x;
-}
-
 // four elements of a row, wherever it begins (those behind column d: zero)
 template <bool BF16>
 __device__ __forceinline__ void row_four(const void* p, int64_t at, int left, float* t) {
@@ -159,13 +148,16 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_k
   if (WAVES == 1 && y >= p.ny) return;
   const int lanes = LSE ? 1 : p.lanes, c = 4 * (lane & (lanes - 1)), left = p.d - c;
   const int at_once = 64 / lanes * WAVES, first = wave * (64 / lanes) + lane / lanes;
-  // the target's row (DQ), the row itself (DT)
+  // what the end needs is asked for first: behind the sums it would be latencies in a row
   int tg = -1;
-  if (!DT) tg = p.target[y];
-  const bool has = !DT && tg >= 0 && tg < p.n_rows;
-  const int64_t row = DT ? y : has ? tg : -1;
-  float t[4] = {0.f, 0.f, 0.f, 0.f};
-  if (!LSE && wave == 0 && row >= 0 && (!DT || p.unit) && left > 0) row_four<BF16>(p.table, row * p.table_stride + c, left, t);
+  float st = 0.f, g = 1.f, factor = 1.f;
+  if (!DT) {
+    tg = p.target[y];
+    st = p.st[y];
+    if (p.weight) g = p.weight[y];
+    if (p.rec) factor = p.fac[y].x;
+  }
+  float t[4] = {0.f, 0.f, 0.f, 0.f};             // the target's row (DQ), the row itself (DT), once the splits' are under way
 
   float m = XENT_NONE, v[4] = {0.f, 0.f, 0.f, 0.f};
   double l = 0.0;
@@ -181,23 +173,27 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_k
       u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (!LSE && in && left > 0) u[i] = *(const float4*)(p.part_o + at * p.pitch + c);
     }
+    if (!LSE && s0 == 0) {                       // (the first lanes of the first wave: those that write the row)
+      const int64_t row = DT ? y : tg >= 0 && tg < p.n_rows ? tg : -1;
+      if (row >= 0 && (!DT || p.unit) && left > 0) row_four<BF16>(p.table, row * p.table_stride + c, left, t);
+    }
     float now = m;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) now = fmaxf(now, pm[i]);
-    const float w0 = exp2f(m - now);
+    const float w0 = __builtin_amdgcn_exp2f(m - now);
     m = now;
     l *= (double)w0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] *= w0;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
-      const float w = exp2f(pm[i] - m);
+      const float w = __builtin_amdgcn_exp2f(pm[i] - m);
       l += (double)pl[i] * (double)w;
       v[0] = fmaf(w, u[i].x, v[0]); v[1] = fmaf(w, u[i].y, v[1]); v[2] = fmaf(w, u[i].z, v[2]); v[3] = fmaf(w, u[i].w, v[3]);
     }
   }
   {
-    const float top = wave_max(m), w = exp2f(m - top);
+    const float top = wave_max(m), w = __builtin_amdgcn_exp2f(m - top);
     m = top;
     if (!DT) l = wave_sum_f64(l * (double)w);
     if (!LSE) {
@@ -220,7 +216,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_k
     for (int k = 0; k < 4; ++k) v[k] = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      const float f = exp2f(redm[w] - m);
+      const float f = __builtin_amdgcn_exp2f(redm[w] - m);
       l += redl[w] * (double)f;
       if (!LSE) {
         const float4 u = *(const float4*)&acc[w][c];
@@ -228,40 +224,40 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_k
       }
     }
   }
-  float half, f, share = 0.f, g = 0.f;      // half * f: the unit's power in two factors, the sums carry the operands' 2^30
+  float lse2, lr, above;
+  float half, f, share = 0.f;               // half * f: the unit's power in two factors, the sums carry the operands' 2^30
   if (!DT) {
-    const double others = (double)m + log2_of(l);           // -inf where the target is the only row
-    double lse2 = others, lr = 0.0, loss = 0.0;
-    if (has) {
-      const double diff = others - (double)p.st[y];          // log2 of (sum of the others / the target's term)
-      const double soft = (double)log1pf(exp2_of(-fabs(diff))) * 1.4426950408889634;
-      lse2 = fmax(others, (double)p.st[y]) + soft;
-      if (diff != diff) lse2 = diff;
-      loss = (fmax(diff, 0.0) + soft) * 0.6931471805599453;
-      lr = fmin(diff, 0.0) - soft;
-      if (diff != diff) loss = lr = diff;
-    } else if (tg >= p.n_rows) {
-      loss = __longlong_as_double(0x7ff8000000000000LL);
-    }
-    g = has ? (p.weight ? p.weight[y] : 1.f) : 0.f;
+    // In base 2: the other rows' sum is 2^(m + lg), -inf where the target is the only row; diff: that sum over the target's term.  Differences
+    // first (m - st is exact where they are close), so that nothing rounds at the size of the logits but lse itself.
+    const bool has = tg >= 0 && tg < p.n_rows;
+    const float lg = log2f((float)l), diff = (m - st) + lg;
+    const float soft = has ? log1pf(exp2f(-fabsf(diff))) * 1.44269504f : 0.f;
+    const bool other = !has || diff > 0.f;                  // the larger of the two
+    const float big = other ? m : st, more = other ? lg + soft : soft;
+    lse2 = big + more;
+    lr = fminf(diff, 0.f) - soft;
+    float loss = has ? (fmaxf(diff, 0.f) + soft) * 0.693147182f : tg >= p.n_rows ? NAN : 0.f;
+    float lse = fmaf(big, 0.693147182f, fmaf(big, -1.90465421e-9f, more * 0.693147182f));      // log 2 in two parts
+    if (has && diff != diff) lse2 = lr = loss = lse = diff;
+    above = other ? -more : (m - st) - more;                // m - lse2
+    if (!has) g = 0.f;
     if (lane == 0) {
-      if (p.loss) p.loss[y] = (float)loss;
-      if (p.lse) p.lse[y] = (float)(lse2 * 0.6931471805599453);
-      p.stat[2 * y] = (float)lse2;
-      p.stat[2 * y + 1] = (float)lr;
+      if (p.loss) p.loss[y] = loss;
+      if (p.lse) p.lse[y] = lse;
+      p.stat[2 * y] = lse2;
+      p.stat[2 * y + 1] = lr;
     }
     if (p.rec && lane < XENT_TR) {      // (the last row: also what fills its tile)
       const int i = (int)(y % XENT_TR), last = y == p.ny - 1 ? XENT_TR - 1 : i;
       if (lane >= i && lane <= last) {
         const bool ok = lane == i;
-        const float k = ok ? p.fac[y].x : 1.f;
-        xent_rec_dt(p.rec[y / XENT_TR], lane, ok, k, BF16 ? 0.f : xent_exponent(k), ok ? tg : -1, ok ? (p.weight ? p.weight[y] : 1.f) : 0.f, (float)lse2,
-                    (float)lr, p.n_rows, p.scale2);
+        const float k = ok ? factor : 1.f;
+        xent_rec_dt(p.rec[y / XENT_TR], lane, ok, k, BF16 ? 0.f : xent_exponent(k), ok ? tg : -1, ok ? g : 0.f, lse2, lr, p.n_rows, p.scale2);
       }
     }
     if (LSE) return;
-    share = exp2_of(lr);
-    half = f = exp2_of(0.5 * ((double)m - lse2));
+    share = exp2f(lr);
+    half = f = exp2f(0.5f * above);
   } else {
     half = exp2f(0.5f * m);
     f = p.scale * half;
@@ -270,7 +266,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_k
   for (int k = 0; k < 4; ++k) v[k] = v[k] * half * f;
   const bool mine = lane < lanes && left > 0;     // (behind the sums every group of `lanes` holds the row)
   float rn = 1.f;
-  if (row >= 0 && p.unit) {
+  if (p.unit) {                                  // (no target: zeros stay zeros)
     const float k = xent_pow2(xent_row_scale(wave_max(fmaxf(fmaxf(fabsf(t[0]), fabsf(t[1])), fmaxf(fabsf(t[2]), fabsf(t[3]))))));
     float ss = 0.f;
 #pragma unroll
