@@ -99,6 +99,17 @@ __device__ __forceinline__ double wave_sum_f64(double x) {
   for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
   return x;
 }
+// 2^x and log2 x of a 64-bit number to float32's relative (absolute, below 1) precision: whole powers apart, the rest in float32
+__device__ __forceinline__ float exp2_of(double x) {
+  const double n = floor(fmax(x, -1000.0));
+  return ldexpf(exp2f((float)(x - n)), (int)n);
+}
+__device__ __forceinline__ double log2_of(double x) {
+  int e;
+  const double f = frexp(x, &e);
+  return x > 0.0 ? (double)(e - 1) + (double)log2f((float)(f + f)) : x == 0.0 ? -INFINITY : x;
+}
+
 // four elements of a row, wherever it begins (those behind column d: zero)
 template <bool BF16>
 __device__ __forceinline__ void row_four(const void* p, int64_t at, int left, float* t) {
@@ -227,19 +238,18 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_k
   float lse2, lr, above;
   float half, f, share = 0.f;               // half * f: the unit's power in two factors, the sums carry the operands' 2^30
   if (!DT) {
-    // In base 2: the other rows' sum is 2^(m + lg), -inf where the target is the only row; diff: that sum over the target's term.  Differences
-    // first (m - st is exact where they are close), so that nothing rounds at the size of the logits but lse itself.
+    // In base 2 and 64 bits: the other rows' sum, -inf where the target is the only row; diff: its log2 over the target's term.  (In 32 bits
+    // 0.2 us less at 100 x 1000 x 128, and the loss twice as far off: 8.5e-7 for 4.4e-7.)
     const bool has = tg >= 0 && tg < p.n_rows;
-    const float lg = log2f((float)l), diff = (m - st) + lg;
-    const float soft = has ? log1pf(exp2f(-fabsf(diff))) * 1.44269504f : 0.f;
-    const bool other = !has || diff > 0.f;                  // the larger of the two
-    const float big = other ? m : st, more = other ? lg + soft : soft;
-    lse2 = big + more;
-    lr = fminf(diff, 0.f) - soft;
-    float loss = has ? (fmaxf(diff, 0.f) + soft) * 0.693147182f : tg >= p.n_rows ? NAN : 0.f;
-    float lse = fmaf(big, 0.693147182f, fmaf(big, -1.90465421e-9f, more * 0.693147182f));      // log 2 in two parts
-    if (has && diff != diff) lse2 = lr = loss = lse = diff;
-    above = other ? -more : (m - st) - more;                // m - lse2
+    const double others = (double)m + log2_of(l), diff = others - (double)st;
+    const double soft = has ? (double)log1pf(exp2_of(-fabs(diff))) * 1.4426950408889634 : 0.0;
+    const double big = has ? fmax(others, (double)st) + soft : others;
+    const bool nan = has && diff != diff;
+    const float loss = nan ? (float)diff : has ? (float)((fmax(diff, 0.0) + soft) * 0.6931471805599453) : tg >= p.n_rows ? NAN : 0.f;
+    const float lse = nan ? loss : (float)(big * 0.6931471805599453);
+    lse2 = nan ? loss : (float)big;
+    lr = nan ? loss : (float)(fmin(diff, 0.0) - soft);
+    above = nan ? loss : (float)((double)m - big);
     if (!has) g = 0.f;
     if (lane == 0) {
       if (p.loss) p.loss[y] = loss;
