@@ -143,6 +143,10 @@ int chain_check(const gqe_chain_args* a, bool backward) {
     return refuse(GQE_ERR_ARG, "%s: a row stride is smaller than dim %d", who, a->dim);
   if (backward && a->n && (a->workspace_bytes < 8 * a->n * a->dim || !a->workspace || !aligned(a->workspace, 4)))
     return refuse(GQE_ERR_WORKSPACE, "%s: needs %lld workspace bytes; got %lld", who, (long long)(8 * a->n * a->dim), (long long)a->workspace_bytes);
+  if (a->n && (backward ? a->dtable == a->table : a->q == a->table)) return refuse(GQE_ERR_ARG, "%s: the result shares memory with the table", who);
+  for (int j = 0; backward && j < a->n_rels; ++j)
+    for (int i = 0; i < a->n_rels; ++i)
+      if (a->drel[j] == a->rel[i]) return refuse(GQE_ERR_ARG, "%s: gradient %d shares memory with relation %d", who, j, i);
   return GQE_OK;
 }
 

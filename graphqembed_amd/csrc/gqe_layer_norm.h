@@ -215,7 +215,7 @@ __global__ __launch_bounds__(LN_THREADS(G)) void gqe_layer_norm_bwd_kernel(LnPas
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        x[c][i] = (x[c][i] - mean) * rstd;             // xhat; columns past the end meet dy = 0
+        x[c][i] = (c * G + t) * N + i < p.d ? (x[c][i] - mean) * rstd : 0.f;      // xhat; past the end it could overflow and meet dy = 0
         dw[c][i] = fmaf(dy[c][i], x[c][i], dw[c][i]);
         db[c][i] += dy[c][i];
         dy[c][i] *= w[c][i];
@@ -394,6 +394,7 @@ int gqe_layer_norm_backward(const gqe_layer_norm_args* a) {
   if (need && (a->workspace_bytes < need || !a->workspace || !aligned(a->workspace, 16)))
     return refuse(GQE_ERR_WORKSPACE, "layer_norm backward: needs %lld workspace bytes, 16-byte aligned; got %lld", (long long)need,
                   (long long)a->workspace_bytes);
+  if (a->dx && (a->dx == a->x || a->dx == a->dy)) return refuse(GQE_ERR_ARG, "layer_norm backward: dx shares memory with x or dy");
   OnDevice dev(a->device);
   if (dev.status != hipSuccess) return hip_refuse(dev.status, "layer_norm backward");
   LnPass p = ln_pass(a);

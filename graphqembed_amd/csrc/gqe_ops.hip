@@ -443,6 +443,8 @@ int gqe_softmax_xent(const gqe_xent_args* a) {
   const XentSpace sp = xent_space(a, pq, pt);
   if (a->workspace_bytes < sp.total || (sp.total && (!a->workspace || !aligned(a->workspace, 256))))
     return refuse(GQE_ERR_WORKSPACE, "softmax_xent: needs %lld workspace bytes, 256-byte aligned; got %lld", (long long)sp.total, (long long)a->workspace_bytes);
+  if ((dq && B && (a->dq == a->q || a->dq == a->table)) || (dt && (a->dtable == a->table || a->dtable == a->q)))
+    return refuse(GQE_ERR_ARG, "softmax_xent: a gradient shares memory with q or table");      // later launches still read both
   OnDevice dev(a->device);
   if (dev.status != hipSuccess) return hip_refuse(dev.status, "softmax_xent");
   hipStream_t stream = (hipStream_t)a->stream;

@@ -10,7 +10,8 @@ entity needs next to it:
 
 ``softmax_xent`` and ``layer_norm`` are differentiable by torch's autograd; the others are the calls a fused training step makes.
 All work is enqueued on ``torch.cuda.current_stream()`` of the tensors' device (which need not be the current device); nothing
-synchronises and nothing is kept between calls, so every call can be captured into a graph.  float32 and bfloat16; sums are
+synchronises and nothing is kept between calls, so every call can be captured into a graph, but for ``softmax_xent`` and
+``layer_norm`` where autograd would record them (they raise: capture the calls they are made of).  float32 and bfloat16; sums are
 float32 (the norm: float64).  There is no CPU fallback: without libgqe.so or a HIP device the calls raise ``GqeLibraryError``.
 """
 from __future__ import annotations
@@ -124,6 +125,16 @@ def _on_gpu(what, *tensors):
     return index
 
 
+def _recorded(what, forms, *tensors):
+    """Whether autograd records a call on these tensors.  Refused in a capture: with an eager graph of the same leaves alive, torch's
+    backward makes that graph's stream wait for the captured one, which ends the capture and the process."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("%s: autograd's form cannot be captured; capture %s" % (what, forms))
+    return True
+
+
 def _dtype(what, t):
     code = _DTYPES.get(t.dtype)
     if code is None:
@@ -227,7 +238,6 @@ def softmax_xent_grads(q, table, target, weight=None, scale=1.0, normalize=False
 class _SoftmaxXent(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, table, target, scale, normalize):
-        _on_gpu("softmax_xent", q, table)
         loss, stat = _floats(q, q.shape[0]), _floats(q, q.shape[0], 2)
         dq, phase = None, XENT_LOSS
         if ctx.needs_input_grad[0]:
@@ -257,7 +267,12 @@ def softmax_xent(q, table, target, scale=1.0, normalize=False, reduction="mean")
     reduction: "none" (loss[n]), "sum", "mean" (over the queries whose target is not ignored; 0 if there is none)."""
     if reduction not in ("none", "sum", "mean"):
         raise ValueError("softmax_xent: reduction %r" % (reduction,))
-    loss = _SoftmaxXent.apply(q, table, target, float(scale), bool(normalize))
+    scale, normalize = float(scale), bool(normalize)
+    _on_gpu("softmax_xent", q, table, target)
+    if _recorded("softmax_xent", "softmax_xent_grads", q, table):
+        loss = _SoftmaxXent.apply(q, table, target, scale, normalize)
+    else:
+        loss = softmax_xent_loss(q, table, target, scale, normalize)[0]
     if reduction == "none":
         return loss
     loss_sum = loss.sum()
@@ -396,7 +411,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Differentiable ``layer_norm_forward`` along the last dimension of x."""
     if x.dim() < 1:
         raise ValueError("layer_norm: a 0-dim tensor")
-    return _LayerNorm.apply(x.reshape(-1, x.shape[-1]), weight, bias, float(eps)).view(x.shape)
+    rows, eps = x.reshape(-1, x.shape[-1]), float(eps)
+    if _recorded("layer_norm", "layer_norm_forward and layer_norm_backward", x, weight, bias):
+        return _LayerNorm.apply(rows, weight, bias, eps).view(x.shape)
+    return layer_norm_forward(rows, weight, bias, eps)[0].view(x.shape)
 
 
 # -- query side of a relation chain ----------------------------------------------------------------------------------------------

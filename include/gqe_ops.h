@@ -7,8 +7,8 @@
  * synchronisation, 0 on success or a negative gqe_status.  The calls need no gqe_ctx and keep no state: every buffer they use is an
  * argument, so calls on different streams (with workspaces of their own) and from different threads are independent, and a call can
  * be captured into a HIP graph (kernels only; the workspace then belongs to that graph, and the first call of a kind, which loads its
- * kernels, comes before).  `device` is the HIP device of the pointers
- * and the stream; it need not be the current one.  gqe_ops_last_error() is the text of the calling thread's last refusal.
+ * kernels, comes before).  `device` is the HIP device of the pointers and the stream; it need not be the current one.  Results and
+ * workspaces share no memory with inputs or with one another (what is scaled or added to in place apart).  gqe_ops_last_error() is the text of the calling thread's last refusal.
  * Rows are `dim` elements with unit stride; row strides are in elements.  Results do not depend on the order of atomics (there are
  * none): the same call on the same inputs gives the same bits. */
 #ifndef GQE_OPS_H

@@ -535,6 +535,44 @@ def test_layer_norm_views_and_autograd():
     assert abs((f(x + h * v) - f(x - h * v)) / (2 * h) - (xa.grad.double() * v.double()).sum().item()) < 0.02
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layer_norm_of_rows_without_spread(dtype):
+    """Equal elements so large that one less the mean of a column past the row's end would overflow: xhat is 0, so dx = (dy - its
+    mean) / sqrt(eps) and the weights' gradients are sums."""
+    from graphqembed_amd import ops
+    for n, d in ((3, 3), (2100, 13)):
+        x = torch.full((n, d), 2.0 ** 122, device="cuda", dtype=dtype)          # (d of them: 2^126, the sums are exact)
+        dy = torch.randn(n, d, device="cuda").to(dtype)
+        y, mean, rstd = ops.layer_norm_forward(x)
+        assert not y.any() and (mean == 2.0 ** 122).all()
+        dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd)
+        e = dy.double()
+        want = (e - e.mean(1, keepdim=True)) * rstd.double()[:, None]
+        half = torch.finfo(dtype).eps / 2
+        # the mean: d + 2 roundings of at most the largest partial sum; then one difference, one product and the result's rounding
+        bound = rstd.double()[:, None] * ((d + 5) * U * e.abs().sum(1, keepdim=True) + 3 * U * e.abs()) + half * want.abs() * 1.01
+        assert ((dx.double() - want).abs() <= bound).all()
+        assert not dw.any() and (db.double() - e.sum(0)).abs().max() <= 2 * n * U * e.abs().sum(0).max()
+
+
+def test_autograd_forms_are_not_captured(monkeypatch):
+    """What autograd would record raises inside a capture; what it would not is the plain call, and works there."""
+    from graphqembed_amd import ops
+    q, table, target, _ = xent_inputs(20, 300, 64, torch.float32, seed=5)
+    qa, w = q.clone().requires_grad_(), torch.ones(64, device="cuda", requires_grad=True)
+    norm = ops.layer_norm(q, w)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in (lambda: ops.softmax_xent(qa, table, target), lambda: ops.softmax_xent(q, table.clone().requires_grad_(), target),
+                 lambda: ops.layer_norm(qa), lambda: ops.layer_norm(q, w), lambda: ops.layer_norm(q, None, w)):
+        with pytest.raises(ValueError, match="captured"):
+            call()
+    with torch.no_grad():
+        got, same = ops.softmax_xent(qa, table, target, reduction="none"), ops.layer_norm(q, w)
+    assert not got.requires_grad and torch.equal(same, norm)
+    loss = ops.softmax_xent_loss(q, table, target)[0]
+    assert torch.equal(got, loss)
+
+
 @pytest.mark.parametrize("n,d,dtype", [(33000, 513, torch.float32), (17000, 1024, torch.float32), (70001, 481, torch.bfloat16)])
 def test_layer_norm_of_large_outputs(n, d, dtype):
     """Outputs that are written past the caches: row for row the bits of a small call, the columns' sums by the formula."""

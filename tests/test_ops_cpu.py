@@ -54,6 +54,36 @@ def test_softmax_xent_refusals(ops, word, change):
     assert word in lib.gqe_ops_last_error().decode()
 
 
+@pytest.mark.parametrize("change", [dict(dq=1 << 20), dict(dq=2 << 20), dict(dtable=1 << 20), dict(dtable=2 << 20)])
+def test_softmax_xent_refuses_gradients_in_the_place_of_inputs(ops, change):
+    lib = ops.library()
+    a = xent_args(ops, **{**dict(q=1 << 20, table=2 << 20, dq=3 << 20, dtable=4 << 20, workspace_bytes=1 << 40), **change})
+    assert lib.gqe_softmax_xent(C.byref(a)) == -1 and "shares memory" in lib.gqe_ops_last_error().decode()
+
+
+@pytest.mark.parametrize("dx", [1 << 20, 2 << 20])
+@pytest.mark.parametrize("n", [10, 5000])
+def test_layer_norm_refuses_gradients_in_the_place_of_inputs(ops, n, dx):
+    lib = ops.library()
+    a = ops.gqe_layer_norm_args()
+    a.dim, a.n_rows, a.x, a.dy, a.dx, a.dweight = 64, n, 1 << 20, 2 << 20, dx, 3 << 20
+    a.mean = a.rstd = a.workspace = 4 << 20
+    a.workspace_bytes, a.x_stride, a.dy_stride, a.dx_stride = 1 << 40, 64, 64, 64
+    assert lib.gqe_layer_norm_backward(C.byref(a)) == -1 and "shares memory" in lib.gqe_ops_last_error().decode()
+
+
+def test_chain_rows_refuse_results_in_the_place_of_inputs(ops):
+    lib = ops.library()
+    a = ops.gqe_chain_args()
+    a.dim, a.n, a.n_rows, a.n_rels, a.rows, a.table, a.table_stride = 64, 4, 9, 2, 8 << 20, 1 << 20, 64
+    a.rel[0], a.rel[1], a.drel[0], a.drel[1] = 2 << 20, 3 << 20, 4 << 20, 5 << 20
+    a.q, a.q_stride, a.dq, a.dq_stride, a.dtable, a.dtable_stride, a.workspace, a.workspace_bytes = 1 << 20, 64, 6 << 20, 64, 1 << 20, 64, 7 << 20, 1 << 30
+    for call in (lib.gqe_chain_rows_forward, lib.gqe_chain_rows_backward):
+        assert call(C.byref(a)) == -1 and "shares memory with the table" in lib.gqe_ops_last_error().decode()
+    a.dtable, a.drel[1] = 9 << 20, 2 << 20
+    assert lib.gqe_chain_rows_backward(C.byref(a)) == -1 and "gradient 1 shares memory with relation 0" in lib.gqe_ops_last_error().decode()
+
+
 def test_null_arguments(ops):
     lib = ops.library()
     assert lib.gqe_softmax_xent(None) == -1 and lib.gqe_softmax_xent_workspace(None) == -1
