@@ -33,7 +33,7 @@ __device__ __forceinline__ void chain_row(const ChainPass& p, int64_t row, int l
     a[c] *= k;             // a power of two: no square over- or underflows
     ss = fmaf(a[c], a[c], ss);
   }
-  const float g = xent_rsqrt(wave_sum(ss));
+  const float g = xent_rsqrt(wave_total(ss));
   rn = fminf(g * k, 3.0e38f);
 #pragma unroll
   for (int c = 0; c < 4; ++c) a[c] *= g;
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void gqe_chain_bwd_kernel(ChainPass p) {
       p.c[(int64_t)b * p.d + i] = g * a[c];
     }
   }
-  along = wave_sum(along);
+  along = wave_total(along);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int i = lane + 64 * c;

@@ -42,7 +42,7 @@ __device__ __forceinline__ int clip_find(const ClipGroup& g, int c) {
 }
 
 __device__ __forceinline__ double clip_block_sum(double x, double* lds) {
-  x = wave_sum_f64(x);
+  x = wave_total(x);
   const int wave = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) lds[wave] = x;
   __syncthreads();
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(CLIP_FEW_THREADS) void gqe_clip_few_kernel(ClipGrou
       else f(u[k], at[k]);
     }
   clip_ragged(g, f, b);
-  const double s = wave_sum_f64((f.s0 + f.s1) + (b.s0 + b.s1));
+  const double s = wave_total((f.s0 + f.s1) + (b.s0 + b.s1));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
   double n = 0.0;

@@ -88,8 +88,13 @@ __device__ __forceinline__ void ln_store(void* row, int col, int d, const float*
 // sums of a and b over the G threads of a row
 template <int G>
 __device__ __forceinline__ void ln_sum2(float& a, float& b, float (*lds)[2]) {
-#pragma unroll
-  for (int o = (G < 64 ? G : 64) / 2; o; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+  if (G >= 64) { a = lane_sum<32>(a); b = lane_sum<32>(b); }
+  if (G >= 32) { a = lane_sum<16>(a); b = lane_sum<16>(b); }
+  if (G >= 16) { a = lane_sum<8>(a); b = lane_sum<8>(b); }
+  if (G >= 16) { a = lane_sum<4>(a); b = lane_sum<4>(b); }
+  else { a += __shfl_xor(a, 4); b += __shfl_xor(b, 4); }      // lanes 8 apart are another row's
+  a = lane_sum<1>(lane_sum<2>(a));
+  b = lane_sum<1>(lane_sum<2>(b));
   if (G > 64) {
     const int wave = threadIdx.x >> 6;
     __syncthreads();                       // the sums before these have been read

@@ -89,15 +89,46 @@ __device__ __forceinline__ void put_elem(void* p, int64_t i, float v, bool accum
   }
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-  return x;
+// f(x of this lane, x of lane ^ O), f commutative, as the arithmetic unit itself moves lanes: a shuffle goes through LDS, 60 cycles and more
+// that nothing hides where a row's sums follow one another.  O = 4: lanes 8 apart hold the same x already (rows of 16 are turned by 4).
+template <int O>
+__device__ __forceinline__ void lane_pair(uint32_t x, uint32_t& a, uint32_t& b) {
+  if (O == 32 || O == 16) {
+    const auto r = O == 32 ? __builtin_amdgcn_permlane32_swap(x, x, false, false) : __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    a = r[0];
+    b = r[1];
+  } else {
+    constexpr int how = O == 8 ? 0x128 : O == 4 ? 0x124 : O == 2 ? 0x4e : 0xb1;      // row_ror:8, row_ror:4, quad_perm [2,3,0,1], [1,0,3,2]
+    a = x;
+    b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, how, 0xf, 0xf, true);
+  }
 }
-__device__ __forceinline__ double wave_sum_f64(double x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+template <int O>
+__device__ __forceinline__ float lane_sum(float x) {
+  uint32_t a, b;
+  lane_pair<O>(__float_as_uint(x), a, b);
+  return __uint_as_float(a) + __uint_as_float(b);
+}
+template <int O>
+__device__ __forceinline__ float lane_max(float x) {
+  uint32_t a, b;
+  lane_pair<O>(__float_as_uint(x), a, b);
+  return fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+template <int O>
+__device__ __forceinline__ double lane_sum(double x) {
+  uint32_t a[2], b[2];
+  lane_pair<O>((uint32_t)__double2loint(x), a[0], b[0]);
+  lane_pair<O>((uint32_t)__double2hiint(x), a[1], b[1]);
+  return __hiloint2double((int)a[1], (int)a[0]) + __hiloint2double((int)b[1], (int)b[0]);
+}
+// over all 64 lanes, the same bits in each
+template <typename T>
+__device__ __forceinline__ T wave_total(T x) {
+  return lane_sum<1>(lane_sum<2>(lane_sum<4>(lane_sum<8>(lane_sum<16>(lane_sum<32>(x))))));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return lane_max<1>(lane_max<2>(lane_max<4>(lane_max<8>(lane_max<16>(lane_max<32>(x))))));
 }
 // 2^x and log2 x of a 64-bit number to float32's relative (absolute, below 1) precision: whole powers apart, the rest in float32
 __device__ __forceinline__ float exp2_of(double x) {
@@ -206,13 +237,18 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_k
   {
     const float top = wave_max(m), w = __builtin_amdgcn_exp2f(m - top);
     m = top;
-    if (!DT) l = wave_sum_f64(l * (double)w);
+    if (!DT) l = wave_total(l * (double)w);
     if (!LSE) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] *= w;
-      for (int o = lanes; o < 64; o <<= 1)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += __shfl_xor(v[k], o);
+      for (int k = 0; k < 4; ++k) {      // lanes that hold the same columns
+        if (lanes <= 32) v[k] = lane_sum<32>(v[k]);
+        if (lanes <= 16) v[k] = lane_sum<16>(v[k]);
+        if (lanes <= 8) v[k] = lane_sum<8>(v[k]);
+        if (lanes <= 4) v[k] = lane_sum<4>(v[k]);
+        if (lanes <= 2) v[k] = lane_sum<2>(v[k]);
+        if (lanes <= 1) v[k] = lane_sum<1>(v[k]);
+      }
     }
   }
   if (WAVES > 1) {
@@ -281,7 +317,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_k
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) ss = fmaf(t[i] * k, t[i] * k, ss);
-    rn = xent_rsqrt(wave_sum(lane < lanes ? ss : 0.f)) * k;
+    rn = xent_rsqrt(wave_total(lane < lanes ? ss : 0.f)) * k;
 #pragma unroll
     for (int i = 0; i < 4; ++i) t[i] *= rn;
   }
@@ -293,7 +329,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_k
     float along = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) along = fmaf(t[i], v[i], along);
-    along = wave_sum(lane < lanes ? along : 0.f);
+    along = wave_total(lane < lanes ? along : 0.f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (v[i] - t[i] * along) * rn;
   }
