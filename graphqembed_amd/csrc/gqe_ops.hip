@@ -422,14 +422,15 @@ void join_launch(bool bf16, const XentJoin& j, hipStream_t s) {
   if (bf16) gqe_xent_join_kernel<true, MODE, WAVES><<<grid, block, 0, s>>>(j);
   else gqe_xent_join_kernel<false, MODE, WAVES><<<grid, block, 0, s>>>(j);
 }
-// A wave a row where it takes the splits in one go (64 / lanes of them, XENT_JOIN_BATCH times) or rows are many (4608 rows of 14 splits of
-// d = 192: eight waves 42 us); else 16, or 8 where there are rows for every CU (229 splits of d = 208: 58 rows 12 us against 18; 512
-// rows of 64 splits 16 us against 11).
+// As many waves a row as take the splits in one go (64 / lanes of them a wave, XENT_JOIN_BATCH times): 1, 4 (1203 rows of 25 splits of d = 217:
+// 10 us, with eight waves 15, fewer rows at once) or 8; 16 where there are not rows for every CU (229 splits of d = 208: 58 rows 12 us against
+// 18; 512 rows of 64 splits 16 us against 11).  One wave anyway where rows are many (4608 rows of 14 splits of d = 192: eight waves 42 us).
 template <int MODE>
 void join_launch(bool bf16, XentJoin j, hipStream_t s) {
   j.lanes = 1;
   while (MODE != XENT_MODE_LSE && 4 * j.lanes < j.d) j.lanes *= 2;
   if (j.n_split * j.lanes <= 64 * XENT_JOIN_BATCH || j.ny > 2048) join_launch<MODE, 1>(bf16, j, s);
+  else if (j.n_split * j.lanes <= 4 * 64 * XENT_JOIN_BATCH) join_launch<MODE, 4>(bf16, j, s);
   else if (j.ny > 256) join_launch<MODE, 8>(bf16, j, s);
   else join_launch<MODE, 16>(bf16, j, s);
 }
