@@ -4,9 +4,9 @@
 // threads (a part of a wave, a wave, or a workgroup), EPL elements each in 16-byte pieces, so mean and variance are two passes
 // over registers (no cancellation) and nothing is read twice.  The weight's and bias's gradients are column sums: each thread
 // keeps its columns' sums over the rows its group takes, a workgroup adds its groups and writes one row of partial sums, a second
-// launch adds the workgroups' rows in order (no atomics: the same bits every time).  500000 x 256 float32: forward 240 us (4.3 TB/s; with the
-// next row under way while one is summed, 2048 workgroups: the same), backward 275 us (5.6 TB/s) + 5 us of column sums, where a copy of
-// that size reaches 4.8 TB/s; 512 x 128: 3.5 + 3.7 us, launches.
+// launch adds the workgroups' rows in order (no atomics: the same bits every time).  500000 x 256 float32: forward 225 us (4.6 TB/s; with the
+// next row under way while one is summed, 2048 workgroups: the same), backward 290 us (5.3 TB/s) + 5 us of column sums, where a copy of
+// that size reaches 4.8 TB/s; 512 x 128: 3.0 + 3.5 us, launches.
 #ifndef GQE_LAYER_NORM_H
 #define GQE_LAYER_NORM_H
 
