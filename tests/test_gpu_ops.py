@@ -555,6 +555,53 @@ def test_layer_norm_of_rows_without_spread(dtype):
         assert not dw.any() and (db.double() - e.sum(0)).abs().max() <= 2 * n * U * e.abs().sum(0).max()
 
 
+def test_a_run_of_operators_in_two_graphs():
+    """Chain rows, layer norm, cross entropy, their backward passes and clipping, captured for two batches whose graphs share a memory
+    pool and replayed in turn, eager steps between them: every replay has the eager bits."""
+    from graphqembed_amd import ops
+    V, d = 700, 96
+    table = torch.randn(V, d, device="cuda")
+    rels = [torch.randn(d, device="cuda") for _ in range(2)]
+    w, b = torch.rand(d, device="cuda") + 0.5, torch.randn(d, device="cuda")
+
+    def step(rows, target):
+        grads = [torch.zeros_like(t) for t in [table] + rels + [w, b]]
+        q = ops.chain_rows(table, rows, rels)
+        y, mean, rstd = ops.layer_norm_forward(q, w, b)
+        loss, lse, dy, _ = ops.softmax_xent_grads(y, table, target, normalize=True, grad_table=grads[0])
+        dq, _, _ = ops.layer_norm_backward(dy, q, mean, rstd, w, grads[3], grads[4])
+        ops.chain_rows_backward(dq, table, rows, rels, grads[0], grads[1:3])
+        small = ops.clip_grad_norm_(grads[1:], 0.1)
+        return [loss, lse, ops.clip_grad_norm_(grads, 0.5), small] + grads
+
+    def batch(n):
+        rows, target = (torch.randint(0, V, (n,), device="cuda", dtype=torch.int32) for _ in range(2))
+        target[::5] = -1
+        return rows, target
+
+    feeds = [batch(150), batch(40)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for f in feeds:
+            step(*f)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for f in feeds:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=graphs[0].pool() if len(graphs) > 1 else None):
+            outs.append(step(*f))
+    for _ in range(3):
+        table.copy_(torch.randn(V, d, device="cuda"))
+        for f, graph, out in zip(feeds, graphs, outs):
+            for into, value in zip(f, batch(len(f[0]))):
+                into.copy_(value)
+            graph.replay()
+            want = step(*f)
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
 def test_autograd_forms_are_not_captured(monkeypatch):
     """What autograd would record raises inside a capture; what it would not is the plain call, and works there."""
     from graphqembed_amd import ops
