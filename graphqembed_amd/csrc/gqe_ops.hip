@@ -177,7 +177,7 @@ __device__ __forceinline__ void put_four(void* p, int64_t at, int left, const fl
 // The splits' sums of a stationary row, each with its own unit 2^part_m, added in a fixed order.  Bound by latency: a lane takes 16 bytes of
 // a split, `lanes` of them a row, so that a wave has 64 / lanes splits at once and eight times as many under way, and nothing waits for
 // the largest unit: each lane's sums follow a running one of their own and are brought together at the end.  WAVES = 1: a wave per row,
-// four rows a workgroup (few splits, many rows); 16: a workgroup per row.
+// four rows a workgroup (few splits, or many rows); more: a workgroup per row.
 template <bool BF16, int MODE, int WAVES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void gqe_xent_join_kernel(XentJoin p) {
   constexpr bool LSE = MODE == XENT_MODE_LSE, DT = MODE == XENT_MODE_DT;
@@ -422,15 +422,18 @@ void join_launch(bool bf16, const XentJoin& j, hipStream_t s) {
   if (bf16) gqe_xent_join_kernel<true, MODE, WAVES><<<grid, block, 0, s>>>(j);
   else gqe_xent_join_kernel<false, MODE, WAVES><<<grid, block, 0, s>>>(j);
 }
-// As many waves a row as take the splits in one go (64 / lanes of them a wave, XENT_JOIN_BATCH times): 1, 4 (1203 rows of 25 splits of d = 217:
-// 10 us, with eight waves 15, fewer rows at once) or 8; 16 where there are not rows for every CU (229 splits of d = 208: 58 rows 12 us against
-// 18; 512 rows of 64 splits 16 us against 11).  One wave anyway where rows are many (4608 rows of 14 splits of d = 192: eight waves 42 us).
+// Waves a row by `loads`, 16 bytes each, that a row takes (64 a wave at once, XENT_JOIN_BATCH of those under way).  One wave for up to 64, and
+// for up to 512 where rows alone fill the CUs (2000 rows of 10 splits of d = 128: 8 us, with four waves 10); four take up to 2048 (100 rows of
+// 16 splits of d = 128: 5.4 us against 7.7 with one; 1203 rows of 25 splits of d = 217: 10 us against 15 with eight, fewer rows at once); else
+// 8, or 16 where there are not rows for every CU (229 splits of d = 208: 58 rows 12 us against 18; 512 rows of 64 splits 16 us against
+// 11).  One wave anyway where rows are many (4608 rows of 14 splits of d = 192: eight waves 42 us).
 template <int MODE>
 void join_launch(bool bf16, XentJoin j, hipStream_t s) {
   j.lanes = 1;
   while (MODE != XENT_MODE_LSE && 4 * j.lanes < j.d) j.lanes *= 2;
-  if (j.n_split * j.lanes <= 64 * XENT_JOIN_BATCH || j.ny > 2048) join_launch<MODE, 1>(bf16, j, s);
-  else if (j.n_split * j.lanes <= 4 * 64 * XENT_JOIN_BATCH) join_launch<MODE, 4>(bf16, j, s);
+  const int64_t loads = (int64_t)j.n_split * j.lanes, wave = 64 * XENT_JOIN_BATCH;
+  if (loads <= 64 || j.ny > 2048 || (loads <= wave && j.ny > 1024)) join_launch<MODE, 1>(bf16, j, s);
+  else if (loads <= 4 * wave) join_launch<MODE, 4>(bf16, j, s);
   else if (j.ny > 256) join_launch<MODE, 8>(bf16, j, s);
   else join_launch<MODE, 16>(bf16, j, s);
 }
