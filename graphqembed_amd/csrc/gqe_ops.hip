@@ -364,11 +364,14 @@ XentPlan xent_plan_queries(const gqe_xent_args* a) { return xent_plan(a->n_queri
 // The table's gradient takes four tiles of queries at least: below that the join costs more than a split saves (136 queries, 14575 rows of
 // d = 200, 5 tiles: 20 us, and a join of 11 us as 4 + 1).  Where float32 rows of d > 64 are converted on the way a tile takes 3 to 8 us, and
 // with three or four of them and few rows to join each goes by itself (100 queries, 1000 rows of d = 128: 20 us, apart 12 + 4; d = 64: 13
-// us, apart 10 + 5).
+// us, apart 10 + 5).  Where tiles are cheap (0.5 to 1.1 us: bfloat16, or d <= 64) and rows to join are many, a workgroup takes up to 19 itself (11
+// tiles, 11988 bfloat16 rows of d = 175: 22 us against 17 + 10 in two splits; 19 tiles, 20000 float32 rows of d = 64: 30 us against 23 + 13 in
+// three; with 8000 rows or d = 128 the two are even, and 32 tiles of d = 64, 12000 rows, are 23 + 10 us in four splits, 27 + 9 in three).
 XentPlan xent_plan_table(const gqe_xent_args* a) {
   const int64_t blocks = (a->n_rows + XENT_BM - 1) / XENT_BM, tiles = (a->n_queries + XENT_TR - 1) / XENT_TR;
   const bool apart = a->dtype == GQE_F32 && a->dim > 64 && !xent_prepares(a) && tiles >= 3 && blocks * tiles <= 128;
-  return xent_plan(a->n_rows, a->n_queries, a->dim, xent_slots(a), apart ? 1 : 4);
+  const bool cheap = (a->dtype == GQE_BF16 || a->dim <= 64) && blocks >= 80 && tiles < 20;
+  return xent_plan(a->n_rows, a->n_queries, a->dim, xent_slots(a), apart ? 1 : cheap ? 20 : 4);
 }
 // bfloat16 rows that are operands as they lie: whole tiles wide, 16-byte pieces
 bool xent_as_is(bool bf16, int dk, int dim, const void* ptr, int64_t stride) { return bf16 && dk == dim && aligned(ptr, 16) && stride % 8 == 0 && stride < (1 << 25); }

@@ -106,6 +106,7 @@ def test_softmax_xent_workspace(ops):
         assert need(n_rows=100000000, n_queries=512, dim=dim, dtype=1) < 100000000 * (padded * 2 + 25) + 2 * parts
     assert need(n_rows=100000000, n_queries=128, dim=256, phase=1) < 1 << 20
     assert need(n_queries=0) == 256
+    assert all(need(n_queries=n, n_rows=rows, dtype=dtype, phase=4, dim=40) > 0 for n in (0, 1, 600, 700) for rows in (1, 10240, 1 << 30) for dtype in (0, 1))
     assert need(n_rows=0x7fffff00, n_queries=0x7fffff00, dim=256, phase=2) > 0       # sizes stay in 64 bits
 
 
